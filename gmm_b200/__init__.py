@@ -150,11 +150,36 @@ def _register_fakes() -> None:
         n = b.shape[1] if trans_b else b.shape[2]
         return torch.empty(a.shape[0], n // 2, dtype=a.dtype, device=a.device)
 
-    try:  # absent only in a stale build; `python -m gmm_b200.build` refreshes it
-        torch.library.register_fake("hopper_gmm_fwd::gmm_swiglu")(_gmm_swiglu_fake)
-    except RuntimeError:
-        warnings.warn("gmm_b200._C predates gmm_swiglu; rebuild with `python -m gmm_b200.build`",
-                      RuntimeWarning)
+    def _gmm_int8_fake(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu):
+        n = b.shape[1] // 2 if swiglu else b.shape[1]
+        return torch.empty(a.shape[0], n, dtype=out_dtype, device=a.device)
+
+    def _quantize_rows_fake(x, dst_pos, out_rows):
+        q = torch.empty(out_rows, (x.shape[1] + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+        return q, torch.empty(out_rows, dtype=torch.float32, device=x.device)
+
+    def _post_norm_fake(y, x, weight, gate, next_weight, gate_act, residual_scale, eps, weight_offset, keep):
+        rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+        stat = [torch.empty(rows if keep and t is not None else 0, dtype=torch.float32, device=x.device)
+                for t in (y, next_weight)]
+        outs = [torch.empty(x.shape if t is not None else (0,), dtype=x.dtype, device=x.device)
+                for t in (y, next_weight)]
+        return outs[0], outs[1], stat[0], stat[1]
+
+    def _post_norm_backward_fake(y, x, weight, gate, next_weight, rstd_y, rstd_x, dx_new, dh, gate_act,
+                                 residual_scale, weight_offset):
+        like = (y, x, weight if y is not None else None, gate, next_weight)
+        return [torch.empty((0,) if t is None else t.shape, dtype=(x if t is None else t).dtype, device=x.device)
+                for t in like]
+
+    for name, fake in (("gmm_swiglu", _gmm_swiglu_fake), ("gmm_int8", _gmm_int8_fake),
+                       ("gmm_int8_dev", _gmm_int8_fake), ("quantize_rows", _quantize_rows_fake),
+                       ("post_norm", _post_norm_fake), ("post_norm_backward", _post_norm_backward_fake)):
+        try:  # absent only in a stale build; `python -m gmm_b200.build` refreshes it
+            torch.library.register_fake(f"hopper_gmm_fwd::{name}")(fake)
+        except RuntimeError:
+            warnings.warn(f"gmm_b200._C predates {name}; rebuild with `python -m gmm_b200.build`",
+                          RuntimeWarning)
 
 
 if not load_native():

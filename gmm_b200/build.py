@@ -25,10 +25,13 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB = os.path.join(PKG, "libgmm_sm100.so")
 TORCH_OP = os.path.join(PKG, "_C.so")
 
-KERNEL_SOURCES = [os.path.join(CSRC, f) for f in ("gmm_sm100.cu", "moe_sm100.cu")]
+KERNEL_SOURCES = [os.path.join(CSRC, f) for f in ("gmm_sm100.cu", "moe_sm100.cu", "quant_sm100.cu",
+                                                       "norm_sm100.cu")]
 KERNEL_HEADERS = [os.path.join(CSRC, "sm100_ptx.cuh"), os.path.join(CSRC, "gmm_pair_kernel.cuh"),
                   os.path.join(CSRC, "gmm_vark_kernel.cuh"),
                   os.path.join(CSRC, "gmm_swap_kernel.cuh"),
+                  os.path.join(CSRC, "row_vec.cuh"),
+                  os.path.join(CSRC, "status.h"),
                   os.path.join(INCLUDE, "gmm_sm100.h")]
 
 
@@ -47,8 +50,9 @@ def _run(cmd, verbose):
 
 def build_kernels(force=False, verbose=True, extra=()):
     if force or _stale(LIB, KERNEL_SOURCES + KERNEL_HEADERS):
-        _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-              "-I", INCLUDE, *extra, "-o", LIB, *KERNEL_SOURCES], verbose)
+        # the sources compile side by side (nvcc --threads)
+        _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--threads", str(len(KERNEL_SOURCES)),
+              "-Xcompiler", "-fPIC", "-shared", "-I", INCLUDE, *extra, "-o", LIB, *KERNEL_SOURCES], verbose)
     return LIB
 
 

@@ -59,6 +59,27 @@ _SIGNATURES = {
                                                ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                                ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
     "gmm_sm100_moe_last_error": (ctypes.c_char_p, []),
+    "gmm_sm100_forward_int8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                              ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "gmm_sm100_int8_workspace_size": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                                        ctypes.c_int64, ctypes.c_int64]),
+    "gmm_sm100_forward_int8_dev": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                  ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+                                                  ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                                  ctypes.c_void_p]),
+    "gmm_sm100_quantize_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                               ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "gmm_sm100_post_norm": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 2 + [ctypes.c_int] * 5
+                            + [ctypes.c_float] * 3 + [ctypes.c_void_p] * 5),
+    "gmm_sm100_post_norm_backward": (ctypes.c_int, [ctypes.c_void_p] * 9 + [ctypes.c_int64] * 2
+                                     + [ctypes.c_int] * 5 + [ctypes.c_float] * 2 + [ctypes.c_void_p] * 6
+                                     + [ctypes.c_size_t, ctypes.c_void_p]),
+    "gmm_sm100_post_norm_backward_workspace_size": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     "gmm_sm100_ep_gather": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int64, ctypes.c_void_p]),

@@ -27,26 +27,31 @@
 // epilogue warp q drains rows 32 (q & 1) .. +31 of column half q >> 1.  The
 // SwiGLU epilogue pairs gate and up columns inside one thread's row, which
 // this layout splits across lanes, so SwiGLU launches keep 256-row tiles.
+//
+// 8-bit operands (kind::i8) keep every byte count above: a k-block is 128
+// deep, an MMA contracts K=32 in the time of a 16-bit K=16, the accumulators
+// are 32-bit integers and the epilogue scales them (AccScaled).
 #pragma once
 
 template <int kKind, bool kBMnMajor>
 struct PairCfg {
-  static_assert(kKind == kKindBf16 || kKind == kKindF16, "pair tiles are 16-bit only");
-  static constexpr int kElem = 2;
+  static_assert(kKind != kKindTf32x3, "pair tiles take 16-bit and 8-bit operands");
+  static_assert(!(is_i8(kKind) && kBMnMajor), "8-bit operands are K-major");
+  static constexpr int kElem = is_i8(kKind) ? 1 : 2;
   static constexpr int BM = 256;      // rows per pair tile
   static constexpr int BM_CTA = 128;  // rows per CTA
   static constexpr int BN = 256;      // output columns per tile
   static constexpr int BN_CTA = 128;  // B columns held by each CTA
-  static constexpr int BK = 64;
+  static constexpr int BK = 128 / kElem;  // one 128-byte swizzle row of K
   static constexpr int kStages = 6;
-  static constexpr int kUmmaK = 16;
+  static constexpr int kUmmaK = 32 / kElem;
   static constexpr int kKSteps = BK / kUmmaK;
   static constexpr int kABytes = BM_CTA * BK * kElem;  // 16 KB
   static constexpr int kBBytes = BN_CTA * BK * kElem;  // 16 KB
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kTmemCols = 2 * BN;
-  static constexpr uint32_t kIdesc = make_idesc(kKind == kKindBf16 ? 1u : 0u, kBMnMajor, BM, BN);
-  static constexpr uint32_t kIdescHalf = make_idesc(kKind == kKindBf16 ? 1u : 0u, kBMnMajor, BM / 2, BN);
+  static constexpr uint32_t kIdesc = kind_idesc<kKind>(kBMnMajor, BM, BN);
+  static constexpr uint32_t kIdescHalf = kind_idesc<kKind>(kBMnMajor, BM / 2, BN);
   static constexpr int kHalfABytes = kABytes / 2;  // 64 A rows per CTA in a half tile
   static constexpr int kBarBytes = 256;
   static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes + 1024;
@@ -209,7 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_pair_kernel(const __grid_cons
             const uint64_t bdesc = kBMnMajor
                                        ? make_sw128_desc(sb + ks * C::kUmmaK * 128, C::BK * 128, 1024)
                                        : make_sw128_desc(sb + ks * 32, 16, 1024);
-            mma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | ks) != 0 ? 1u : 0u);
+            if constexpr (is_i8(kKind))
+              mma_i8_pair(d_tmem, adesc, bdesc, idesc, (kb | ks) != 0 ? 1u : 0u);
+            else
+              mma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb | ks) != 0 ? 1u : 0u);
           }
           mma_commit_pair_mc(smem_u32(empty_bar + stage), 0x3);
           if (++stage == C::kStages) {
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_pair_kernel(const __grid_cons
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    using OutT = typename std::conditional<kKind == kKindBf16, __nv_bfloat16, __half>::type;
+    using OutT = KindOut<kKind>;
     const int quarter = warp & 3;
     const uint32_t stage = smem_u32(epi_stage) + quarter * (32 * 128);
     const uint32_t tempty_leader0 = map_shared_to_rank(smem_u32(tempty_bar), 0);
@@ -244,19 +252,20 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_pair_kernel(const __grid_cons
         const int rows_cta = t.rows - (C::BM_CTA / 2) * static_cast<int>(cta);
         const int rb = (quarter & 1) * 32;
         if (rb < rows_cta)  // warp-uniform
-          drain_slab<OutT, C::BN / 2>(p, tv, g, t.row0 + (C::BM_CTA / 2) * static_cast<int>(cta) + rb,
+          drain_slab<OutT, C::BN / 2, is_i8(kKind)>(p, tv, g, t.row0 + (C::BM_CTA / 2) * static_cast<int>(cta) + rb,
                                       min(32, rows_cta - rb), t.n0 + (quarter >> 1) * (C::BN / 2), taddr,
                                       stage, lane);
       } else {
         const int rows_cta = t.rows - C::BM_CTA * static_cast<int>(cta);
         const int row0 = t.row0 + C::BM_CTA * static_cast<int>(cta);
         if (quarter * 32 < rows_cta) {  // warp-uniform
-          if (p.act)
-            drain_slab_swiglu<OutT>(p, tv, g, row0 + quarter * 32, min(32, rows_cta - quarter * 32),
-                                    t.n0 >> 1, taddr, stage, lane);
-          else
-            drain_slab<OutT, C::BN>(p, tv, g, row0 + quarter * 32, min(32, rows_cta - quarter * 32), t.n0,
-                                    taddr, stage, lane);
+          const int slab0 = row0 + quarter * 32, rows = min(32, rows_cta - quarter * 32);
+          if (sizeof(OutT) == 2 && p.act) {
+            if constexpr (sizeof(OutT) == 2)
+              drain_slab_swiglu<OutT, is_i8(kKind)>(p, tv, g, slab0, rows, t.n0 >> 1, taddr, stage, lane);
+          } else {
+            drain_slab<OutT, C::BN, is_i8(kKind)>(p, tv, g, slab0, rows, t.n0, taddr, stage, lane);
+          }
         }
       }
       tc_fence_before();

@@ -44,6 +44,7 @@
 
 #include "gmm_sm100.h"
 #include "sm100_ptx.cuh"
+#include "status.h"
 
 namespace gmm_sm100 {
 
@@ -99,6 +100,10 @@ struct __align__(64) GmmParamsBase {
   int drop_kb1;
   void* d_peer[kMaxPeers];  // each rank's output buffer (remote mode)
   int inline_ints;          // ints of inline_table in use (0: the table is in ext_table or built on device)
+  // 8-bit integer operands: D[i][n] = scale_a[i] * scale_b[expert * scale_cols + n] * (integer sum).
+  const float* scale_a;  // one per row of A
+  const float* scale_b;  // one per expert and output column (gate and up columns for SwiGLU)
+  long long scale_cols;  // columns of scale_b (= of B)
 };
 
 // Kernel parameters: the fields above plus the inline table, in two sizes.  A
@@ -123,17 +128,32 @@ constexpr int kSmallTableInts = 3 * kSmallGroups + 2;
 using GmmParams = GmmParamsT<kInlineTableInts>;
 using GmmParamsSmall = GmmParamsT<kSmallTableInts>;
 
-enum Kind : int { kKindTf32x3 = 0, kKindBf16 = 1, kKindF16 = 2 };
+// The 8-bit kinds share operands and MMAs and differ in the output type.
+enum Kind : int {
+  kKindTf32x3 = 0, kKindBf16 = 1, kKindF16 = 2, kKindI8ToBf16 = 3, kKindI8ToF16 = 4, kKindI8ToF32 = 5
+};
+__host__ __device__ constexpr bool is_i8(int kind) { return kind >= kKindI8ToBf16; }
+template <int kKind>
+using KindOut = typename std::conditional<
+    kKind == kKindTf32x3 || kKind == kKindI8ToF32, float,
+    typename std::conditional<kKind == kKindBf16 || kKind == kKindI8ToBf16, __nv_bfloat16, __half>::type>::type;
+// Instruction descriptor of an M x N MMA of the kind.
+template <int kKind>
+__host__ __device__ constexpr uint32_t kind_idesc(bool b_mn_major, int M, int N) {
+  return is_i8(kKind) ? make_idesc_i8(M, N)
+                      : make_idesc(kKind == kKindTf32x3 ? 2u : (kKind == kKindBf16 ? 1u : 0u), b_mn_major, M, N);
+}
 
 template <int kKind, bool kBMnMajor>
 struct Cfg {
   static constexpr bool kTf32 = (kKind == kKindTf32x3);
-  static constexpr int kElem = kTf32 ? 4 : 2;
+  static constexpr int kElem = kTf32 ? 4 : (is_i8(kKind) ? 1 : 2);
+  static_assert(!(is_i8(kKind) && kBMnMajor), "8-bit operands are K-major");
   static constexpr int BM = 128;
   static constexpr int BN = kTf32 ? 128 : 256;
   static constexpr int BK = 128 / kElem;  // one 128-byte swizzle row of K
   static constexpr int kStages = kTf32 ? 3 : 4;
-  static constexpr int kUmmaK = 32 / kElem;  // K per tcgen05.mma: 16 (16-bit), 8 (tf32)
+  static constexpr int kUmmaK = 32 / kElem;  // K per tcgen05.mma: 16 (16-bit), 8 (tf32), 32 (8-bit)
   static constexpr int kKSteps = BK / kUmmaK;
   static constexpr int kParts = kTf32 ? 2 : 1;  // hi/lo operand copies
   static constexpr int kABytes = BM * BK * kElem;
@@ -142,8 +162,7 @@ struct Cfg {
   static constexpr int kLoadBytes = kABytes + kBBytes;  // bytes TMA brings in per stage
   static constexpr int kPanelCols = 128 / kElem;        // MN-major B: columns per 128-byte panel
   static constexpr int kTmemCols = 2 * BN;  // double-buffered fp32 accumulator
-  static constexpr uint32_t kIdesc =
-      make_idesc(kTf32 ? 2u : (kKind == kKindBf16 ? 1u : 0u), kBMnMajor, BM, BN);
+  static constexpr uint32_t kIdesc = kind_idesc<kKind>(kBMnMajor, BM, BN);
   static constexpr int kBarBytes = 256;
   static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes + 1024;
   static_assert(kABytes % 1024 == 0 && kBBytes % 1024 == 0, "swizzle atoms need 1 KB alignment");
@@ -327,12 +346,37 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Drains one 32-row slab of an accumulator -- TMEM lanes [32q, 32q + 32) of
-// columns [taddr, taddr + BN) -- into its output rows.  Each thread converts its
-// own row; the rows then pass through `stage` (32 rows x 128 B, 16-byte chunks
-// XOR-swizzled by row, conflict-free both ways) so that every store
-// instruction writes four whole 128-byte row segments (8 lanes per row): full
-// L2 lines locally, and large NVLink writes when the row lives on a peer.
+// How an accumulator word becomes a number.  Floating-point kinds: its bits.
+struct AccBits {
+  __device__ __forceinline__ void load(int, int) {}
+  __device__ __forceinline__ float get(uint32_t v, int) const { return __uint_as_float(v); }
+};
+// 8-bit kinds: the integer sum times its row's and its column's scale.  The
+// sum (below 2^31) rounds to 24 bits once, and the products once each, so the
+// result is within 3 half-steps of fp32 before the one rounding to the output
+// type.  Every lane of a warp works on the same 32 columns, so load() fetches
+// their scales as eight uniform 16-byte loads; columns from `end` on (past
+// dim_out, a multiple of 4) are not read.
+struct AccScaled {
+  float row;
+  const float* col;  // scales of the expert's columns
+  float c[32];
+  __device__ __forceinline__ void load(int c0, int end) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (c0 + 4 * q < end) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(col + c0 + 4 * q));
+        c[4 * q] = f.x;
+        c[4 * q + 1] = f.y;
+        c[4 * q + 2] = f.z;
+        c[4 * q + 3] = f.w;
+      }
+  }
+  __device__ __forceinline__ float get(uint32_t v, int i) const {
+    return __int2float_rn(static_cast<int>(v)) * row * c[i];
+  }
+};
+
 // Drains one 32-row slab of an accumulator -- TMEM lanes [32q, 32q + 32) of
 // columns [taddr, taddr + BN) -- into the rows rp[] (8 per lane: rows
 // i*4 + lane/8; null = not stored).  Each thread converts its own row; the rows
@@ -341,9 +385,9 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 // whole 128-byte row segments (8 lanes per row): full L2 lines locally, and
 // large NVLink writes when the row lives on a peer.  zero = store zeros
 // without reading TMEM (a tile whose contraction is empty).
-template <typename OutT, int BN>
+template <typename OutT, int BN, typename Acc = AccBits>
 __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim_out, uint32_t taddr,
-                                           uint32_t stage, int lane, bool zero = false) {
+                                           uint32_t stage, int lane, bool zero = false, Acc acc = Acc()) {
   constexpr int kColsPerSeg = 128 / static_cast<int>(sizeof(OutT));  // 64 (16-bit) or 32 (fp32)
   constexpr int kElemsPer16 = 16 / static_cast<int>(sizeof(OutT));
   const int ch = lane & 7;
@@ -357,6 +401,7 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
       uint32_t v[32];
       if (!zero) {
         tmem_ld_32x32b_x32(taddr + c0 + h * 32, v);
+        acc.load(col + h * 32, dim_out);
         tmem_wait_ld();
       } else {
 #pragma unroll
@@ -366,17 +411,20 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 pk;
-          pk.x = pack2<OutT>(__uint_as_float(v[8 * q + 0]), __uint_as_float(v[8 * q + 1]));
-          pk.y = pack2<OutT>(__uint_as_float(v[8 * q + 2]), __uint_as_float(v[8 * q + 3]));
-          pk.z = pack2<OutT>(__uint_as_float(v[8 * q + 4]), __uint_as_float(v[8 * q + 5]));
-          pk.w = pack2<OutT>(__uint_as_float(v[8 * q + 6]), __uint_as_float(v[8 * q + 7]));
+          pk.x = pack2<OutT>(acc.get(v[8 * q + 0], 8 * q + 0), acc.get(v[8 * q + 1], 8 * q + 1));
+          pk.y = pack2<OutT>(acc.get(v[8 * q + 2], 8 * q + 2), acc.get(v[8 * q + 3], 8 * q + 3));
+          pk.z = pack2<OutT>(acc.get(v[8 * q + 4], 8 * q + 4), acc.get(v[8 * q + 5], 8 * q + 5));
+          pk.w = pack2<OutT>(acc.get(v[8 * q + 6], 8 * q + 6), acc.get(v[8 * q + 7], 8 * q + 7));
           st_shared_v4(my_row + (((h * 4 + q) ^ (lane & 7)) << 4), pk);
         }
       } else {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           st_shared_v4(my_row + ((q ^ (lane & 7)) << 4),
-                       make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+                       make_uint4(__float_as_uint(acc.get(v[4 * q], 4 * q)),
+                                  __float_as_uint(acc.get(v[4 * q + 1], 4 * q + 1)),
+                                  __float_as_uint(acc.get(v[4 * q + 2], 4 * q + 2)),
+                                  __float_as_uint(acc.get(v[4 * q + 3], 4 * q + 3))));
       }
     }
     __syncwarp();
@@ -391,8 +439,17 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
   }
 }
 
+// The scales of a slab: lane l's row is slab_row0 + l.
+__device__ __forceinline__ AccScaled slab_scales(const GmmParamsBase& p, int expert, int slab_row0,
+                                                 int slab_rows, int lane) {
+  AccScaled a;
+  a.row = lane < slab_rows ? __ldg(p.scale_a + slab_row0 + lane) : 0.f;
+  a.col = p.scale_b + expert * p.scale_cols;
+  return a;
+}
+
 // drain_rows for a slab of grouped-GEMM rows: destinations from out_row().
-template <typename OutT, int BN>
+template <typename OutT, int BN, bool kI8 = false>
 __device__ __forceinline__ void drain_slab(const GmmParamsBase& p, const TableView& tv, int g,
                                            int slab_row0, int slab_rows, int n0, uint32_t taddr,
                                            uint32_t stage, int lane) {
@@ -402,7 +459,11 @@ __device__ __forceinline__ void drain_slab(const GmmParamsBase& p, const TableVi
     const int rr = i * 4 + (lane >> 3);
     rp[i] = rr < slab_rows ? out_row<OutT>(p, tv, g, slab_row0 + rr) : nullptr;
   }
-  drain_rows<OutT, BN>(rp, n0, p.dim_out, taddr, stage, lane);
+  if constexpr (kI8)
+    drain_rows<OutT, BN, AccScaled>(rp, n0, p.dim_out, taddr, stage, lane, false,
+                                    slab_scales(p, tv.expert[g], slab_row0, slab_rows, lane));
+  else
+    drain_rows<OutT, BN>(rp, n0, p.dim_out, taddr, stage, lane);
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
@@ -410,7 +471,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 // SwiGLU variant of drain_slab: TMEM columns [0, 128) hold the tile's gate
 // projections and [128, 256) the matching up projections; writes
 // silu(gate) * up (fp32) rounded to the output type, 128 columns per tile.
-template <typename OutT>
+template <typename OutT, bool kI8 = false>
 __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const TableView& tv, int g,
                                                   int slab_row0, int slab_rows, int n0, uint32_t taddr,
                                                   uint32_t stage, int lane) {
@@ -420,6 +481,13 @@ __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const 
   for (int i = 0; i < 8; ++i) {
     const int rr = i * 4 + (lane >> 3);
     rp[i] = rr < slab_rows ? out_row<OutT>(p, tv, g, slab_row0 + rr) : nullptr;
+  }
+  using Acc = typename std::conditional<kI8, AccScaled, AccBits>::type;
+  Acc ag, au;  // gate and up
+  if constexpr (kI8) {
+    ag = slab_scales(p, tv.expert[g], slab_row0, slab_rows, lane);
+    au = ag;
+    au.col += p.act_cols;
   }
   const int ch = lane & 7;
   const uint32_t my_row = stage + lane * 128;
@@ -432,13 +500,15 @@ __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const 
       uint32_t gv[32], uv[32];
       tmem_ld_32x32b_x32(taddr + c0 + h * 32, gv);
       tmem_ld_32x32b_x32(taddr + 128 + c0 + h * 32, uv);
+      ag.load(col + h * 32, p.dim_out);
+      au.load(col + h * 32, p.dim_out);
       tmem_wait_ld();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float a[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          a[j] = silu_mul(__uint_as_float(gv[8 * q + j]), __uint_as_float(uv[8 * q + j]));
+          a[j] = silu_mul(ag.get(gv[8 * q + j], 8 * q + j), au.get(uv[8 * q + j], 8 * q + j));
         uint4 pk;
         pk.x = pack2<OutT>(a[0], a[1]);
         pk.y = pack2<OutT>(a[2], a[3]);
@@ -696,6 +766,8 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_persistent_kernel(const __gri
               mma_tf32_ss(d_tmem, adesc, bdesc, C::kIdesc, acc_flag);    // hi * hi
               mma_tf32_ss(d_tmem, adesc, bdesc_lo, C::kIdesc, 1u);      // hi * lo
               mma_tf32_ss(d_tmem, adesc_lo, bdesc, C::kIdesc, 1u);      // lo * hi
+            } else if constexpr (is_i8(kKind)) {
+              mma_i8_ss(d_tmem, adesc, bdesc, C::kIdesc, acc_flag);
             } else {
               mma_f16_ss(d_tmem, adesc, bdesc, C::kIdesc, acc_flag);
             }
@@ -720,8 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_persistent_kernel(const __gri
     // cannot be ready before the last stage is split).
     if (C::kTf32 && conv_warps == 6) split_stages();
     // ------------------------------------------------------------ epilogue
-    using OutT = typename std::conditional<C::kTf32, float,
-        typename std::conditional<kKind == kKindBf16, __nv_bfloat16, __half>::type>::type;
+    using OutT = KindOut<kKind>;
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
     const uint32_t stage = smem_u32(epi_stage) + quarter * (32 * 128);
     int g = 0;
@@ -734,17 +805,12 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_persistent_kernel(const __gri
       const Tile t = decode_tile<C::BM, C::BN>(tv, n_tiles, tile, g);
       if (quarter * 32 < t.rows) {  // warp-uniform: some row of this quarter is live
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::BN;
-        if constexpr (!C::kTf32) {
-          if (p.act) {
-            drain_slab_swiglu<OutT>(p, tv, g, t.row0 + quarter * 32, min(32, t.rows - quarter * 32),
-                                    t.n0 >> 1, taddr, stage, lane);
-          } else {
-            drain_slab<OutT, C::BN>(p, tv, g, t.row0 + quarter * 32, min(32, t.rows - quarter * 32),
-                                    t.n0, taddr, stage, lane);
-          }
+        const int row0 = t.row0 + quarter * 32, rows = min(32, t.rows - quarter * 32);
+        if (sizeof(OutT) == 2 && p.act) {
+          if constexpr (sizeof(OutT) == 2)
+            drain_slab_swiglu<OutT, is_i8(kKind)>(p, tv, g, row0, rows, t.n0 >> 1, taddr, stage, lane);
         } else {
-          drain_slab<OutT, C::BN>(p, tv, g, t.row0 + quarter * 32, min(32, t.rows - quarter * 32), t.n0,
-                                  taddr, stage, lane);
+          drain_slab<OutT, C::BN, is_i8(kKind)>(p, tv, g, row0, rows, t.n0, taddr, stage, lane);
         }
       }
       tc_fence_before();
@@ -891,9 +957,10 @@ struct DeviceInfo {
   int cc_major = 0, cc_minor = 0;
   // Bit per kernel variant whose shared-memory attribute is set: 0 fp32;
   // 1-4 128-row bf16/fp16 x NT/NN; 5-8 CTA pair; 9-10 variable-K bf16/fp16;
-  // 11-14 swap-AB bf16/fp16 x NT/NN.
-  std::atomic<unsigned> smem_attr_set{0};
-  int pair_clusters[16] = {};               // resident CTA pairs per pair-kernel variant
+  // 11-14 swap-AB bf16/fp16 x NT/NN; 32-34 128-row, 35-37 CTA pair with 8-bit
+  // operands and bf16/fp16/fp32 output.  Small-table instantiations: bit + 16.
+  std::atomic<unsigned long long> smem_attr_set{0};
+  int pair_clusters[64] = {};               // resident CTA pairs per pair-kernel variant
 };
 DeviceInfo g_dev[kMaxDevices];
 std::mutex g_dev_mu;
@@ -930,15 +997,22 @@ struct Plan {
 
 int elem_size(int dtype) { return dtype == GMM_DTYPE_F32 ? 4 : 2; }
 
+// Largest contraction of 8-bit operands whose sum cannot leave 32 bits:
+// 128 * 128 * 131071 < 2^31.
+constexpr int64_t kMaxI8Dim = 131071;
+
+// i8: 8-bit operands; dtype is then the output type.
 int make_plan(const int64_t* bs, int64_t E, int64_t T, int64_t K, int64_t N, int dtype, Plan& pl,
-              int64_t tile_rows = 128) {
+              int64_t tile_rows = 128, bool i8 = false) {
   if (E < 0 || T < 0 || K < 0 || N < 0) return fail(GMM_ERR_INVALID_ARGUMENT, "negative size");
   if (E > 0 && !bs) return fail(GMM_ERR_INVALID_ARGUMENT, "batch_sizes is null");
   if (dtype != GMM_DTYPE_F32 && dtype != GMM_DTYPE_BF16 && dtype != GMM_DTYPE_F16)
     return fail(GMM_ERR_DTYPE, "Unsupported dtype: only FP32 / BF16 / FP16 are supported");
+  if (i8 && K > kMaxI8Dim)
+    return fail(GMM_ERR_TOO_LARGE, "8-bit operands take dim <= 131071 (the sums are 32-bit integers)");
   const int64_t BM = tile_rows;
-  const int64_t BN = dtype == GMM_DTYPE_F32 ? 128 : 256;
-  const int64_t BK = dtype == GMM_DTYPE_F32 ? 32 : 64;
+  const int64_t BN = dtype == GMM_DTYPE_F32 && !i8 ? 128 : 256;
+  const int64_t BK = i8 ? 128 : (dtype == GMM_DTYPE_F32 ? 32 : 64);
   int64_t sum = 0, groups = 0, mtiles = 0;
   for (int64_t e = 0; e < E; ++e) {
     if (bs[e] < 0) return fail(GMM_ERR_INVALID_ARGUMENT, "batch_sizes[" + std::to_string(e) + "] is negative");
@@ -999,10 +1073,10 @@ int encode(CUtensorMap* m, CUtensorMapDataType type, int rank, const void* ptr,
 template <typename P>
 int launch_with(void (*kern)(P), const P& prm, int grid, int smem, cudaStream_t stream, DeviceInfo* di, int bit,
                 const char* what) {
-  if (!(di->smem_attr_set.load() & (1u << bit))) {
+  if (!(di->smem_attr_set.load() & (1ull << bit))) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-    di->smem_attr_set.fetch_or(1u << bit);
+    di->smem_attr_set.fetch_or(1ull << bit);
   }
   kern<<<grid, kThreads, smem, stream>>>(prm);
   cudaError_t e = cudaGetLastError();
@@ -1027,8 +1101,7 @@ int check_table(const GmmParams& prm) {
   return GMM_OK;
 }
 
-// Small-table instantiations use bit + 16 of smem_attr_set (bits 0-15 are
-// taken by the full-table variants and the pair and variable-K kernels).
+// Small-table instantiations use bit + 16 of smem_attr_set.
 template <int kKind, bool kMn>
 int launch_variant(const GmmParams& prm, int grid, cudaStream_t stream, DeviceInfo* di, int bit) {
   using C = Cfg<kKind, kMn>;
@@ -1058,7 +1131,7 @@ int launch_pair(const GmmParams& prm, int total_tiles, cudaStream_t stream, Devi
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (!(di->smem_attr_set.load() & (1u << bit))) {
+  if (!(di->smem_attr_set.load() & (1ull << bit))) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(pair)");
     cfg.gridDim = dim3(2 * std::max(1, di->sm_count / 2), 1, 1);
@@ -1066,7 +1139,7 @@ int launch_pair(const GmmParams& prm, int total_tiles, cudaStream_t stream, Devi
     e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
     if (e != cudaSuccess || clusters <= 0) clusters = di->sm_count / 2;
     di->pair_clusters[bit] = clusters;
-    di->smem_attr_set.fetch_or(1u << bit);
+    di->smem_attr_set.fetch_or(1ull << bit);
   }
   const int pairs = std::max(1, std::min(total_tiles, di->pair_clusters[bit]));
   cfg.gridDim = dim3(2 * pairs, 1, 1);
@@ -1114,9 +1187,9 @@ int tile_force() {
   return g_tile_force.load(std::memory_order_relaxed);
 }
 
-TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int dtype, int act, bool remote) {
-  if (dtype == GMM_DTYPE_F32) return kTile128;
-  const bool swap_ok = !act && !remote;
+TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int dtype, int act, bool remote, bool i8) {
+  if (dtype == GMM_DTYPE_F32 && !i8) return kTile128;
+  const bool swap_ok = !act && !remote && !i8;
   const int force = tile_force();
   if (force == GMM_TILE_128) return kTile128;
   if (force == GMM_TILE_PAIR) return kTilePair;
@@ -1172,10 +1245,20 @@ bool append_ep_table(Plan& pl, const int64_t* local_bs, int64_t E, const EpRoute
 // caps the grid (the tile count when the host knows it).
 int setup_and_launch(GmmParams& prm, const void* A, const void* B, int64_t T, int64_t K, int64_t N, int64_t E,
                      int dtype, int trans_b, int64_t tile_rows, int act, int grid_tiles, DeviceInfo* di,
-                     cudaStream_t stream, bool swap = false) {
+                     cudaStream_t stream, bool swap = false, bool i8 = false) {
   int rc = GMM_OK;
   const cuuint64_t uT = T, uK = K, uN = N, uE = E;
-  if (dtype == GMM_DTYPE_F32) {  // raw fp32 operands; the kernel splits them into TF32 hi/lo in shared memory
+  if (i8) {  // A and B[e] ([N, K]) are K-major: boxes of 128 bytes of K, rows as for the 16-bit kinds
+    const CUtensorMapDataType tt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const cuuint64_t adims[2] = {uK, uT}, astr[1] = {uK};
+    const cuuint32_t abox[2] = {128, 128}, abox_half[2] = {128, 64};
+    const cuuint64_t bdims[3] = {uK, uN, uE}, bstr[2] = {uK, uN * uK};
+    const cuuint32_t bbox[3] = {128, (tile_rows == 256 || act) ? 128u : 256u, 1};
+    if ((rc = encode(&prm.tmap_a, tt, 2, A, adims, astr, abox)) ||
+        (tile_rows == 256 && (rc = encode(&prm.tmap_a2, tt, 2, A, adims, astr, abox_half))) ||
+        (rc = encode(&prm.tmap_b, tt, 3, B, bdims, bstr, bbox)))
+      return rc;
+  } else if (dtype == GMM_DTYPE_F32) {  // raw fp32 operands; the kernel splits them into TF32 hi/lo in shared memory
     const cuuint64_t adims[2] = {uK, uT}, astr[1] = {uK * 4};
     const cuuint32_t abox[2] = {32, 128};
     if ((rc = encode(&prm.tmap_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, A, adims, astr, abox))) return rc;
@@ -1212,6 +1295,16 @@ int setup_and_launch(GmmParams& prm, const void* A, const void* B, int64_t T, in
   }
 
   const int grid = std::max(1, std::min(grid_tiles, di->sm_count));
+  if (i8) {
+    if (tile_rows == 256) {
+      if (dtype == GMM_DTYPE_BF16) return launch_pair<kKindI8ToBf16, false>(prm, grid_tiles, stream, di, 35);
+      if (dtype == GMM_DTYPE_F16) return launch_pair<kKindI8ToF16, false>(prm, grid_tiles, stream, di, 36);
+      return launch_pair<kKindI8ToF32, false>(prm, grid_tiles, stream, di, 37);
+    }
+    if (dtype == GMM_DTYPE_BF16) return launch_variant<kKindI8ToBf16, false>(prm, grid, stream, di, 32);
+    if (dtype == GMM_DTYPE_F16) return launch_variant<kKindI8ToF16, false>(prm, grid, stream, di, 33);
+    return launch_variant<kKindI8ToF32, false>(prm, grid, stream, di, 34);
+  }
   if (dtype == GMM_DTYPE_F32)
     return trans_b ? launch_variant<kKindTf32x3, false>(prm, grid, stream, di, 0)
                    : launch_variant<kKindTf32x3, true>(prm, grid, stream, di, 15);
@@ -1244,18 +1337,20 @@ struct PlanObj {
   int64_t tile_rows = 128;
   int64_t E = 0, T = 0, K = 0, N = 0;
   int dtype = 0, trans_b = 0;
+  bool i8 = false;
 };
 
 int plan_impl(const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens, int64_t dim,
-              int64_t dim_out, int dtype, int trans_b, int act, bool remote, PlanObj& po) {
+              int64_t dim_out, int dtype, int trans_b, int act, bool remote, PlanObj& po, bool i8 = false) {
   NvtxRange range("gmm_sm100 plan");
-  int rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl);
+  int rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl, 128, i8);
   if (rc != GMM_OK) return rc;
-  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dtype, act, remote);
+  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dtype, act, remote, i8);
   po.tile_rows = po.kind == kTilePair ? 256 : 128;
-  if (po.tile_rows != 128 &&
-      (rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl, po.tile_rows)) != GMM_OK)
+  if (po.tile_rows != 128 && (rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl,
+                                             po.tile_rows, i8)) != GMM_OK)
     return rc;
+  po.i8 = i8;
   po.E = num_experts;
   po.T = num_tokens;
   po.K = dim;
@@ -1271,11 +1366,24 @@ struct InjectTimeout {
   unsigned long long wait_ns;
 };
 
+// Scales of 8-bit operands.
+struct I8Scales {
+  const float* a;  // [T]
+  const float* b;  // [E, N]
+};
+
+int check_scales(const I8Scales& q) {
+  if (!q.a || !q.b) return fail(GMM_ERR_INVALID_ARGUMENT, "scale_a or scale_b is null");
+  if ((reinterpret_cast<uintptr_t>(q.a) & 3u) || !aligned16(q.b))
+    return fail(GMM_ERR_ALIGNMENT, "scale_a must be 4-byte and scale_b 16-byte aligned");
+  return GMM_OK;
+}
+
 // The device half: argument checks that need the pointers, tensor maps, launch.
 // `pl` is the plan's table (with the expert-parallel segments appended in EP mode).
 int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B, void* D, void* workspace,
                 size_t workspace_bytes, void* stream_ptr, const EpRoute* ep, int act,
-                const InjectTimeout* inject = nullptr) {
+                const InjectTimeout* inject = nullptr, const I8Scales* q = nullptr) {
   NvtxRange range("gmm_sm100 launch");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   int rc = GMM_OK;
@@ -1284,7 +1392,8 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
   const int64_t T = po.T, K = po.K, N = po.N, E = po.E;
   const int dtype = po.dtype, trans_b = po.trans_b;
   if (T == 0 || N == 0) return GMM_OK;  // nothing to write
-  const int es = elem_size(dtype);
+  const int es = elem_size(dtype);        // of D
+  const int in_es = po.i8 ? 1 : es;       // of A and B
   // SwiGLU: B has 2*I output columns ([gate | up]); D has I = N / 2 columns.
   const int64_t N_out = act ? N / 2 : N;
   if (act) {
@@ -1292,6 +1401,7 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
     if (N % 16 != 0)
       return fail(GMM_ERR_ALIGNMENT, "SwiGLU needs the gate/up width (dim_out / 2) to be a multiple of 8");
   }
+  if (q && (rc = check_scales(*q)) != GMM_OK) return rc;
   if (ep) {
     if (ep->world < 1 || ep->world > kMaxPeers || !ep->out_peers)
       return fail(GMM_ERR_INVALID_ARGUMENT, "expert-parallel world must be 1.." + std::to_string(kMaxPeers));
@@ -1317,7 +1427,7 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
   }
   if (!A || !B) return fail(GMM_ERR_INVALID_ARGUMENT, "A or B is null");
   if (!aligned16(A) || !aligned16(B)) return fail(GMM_ERR_ALIGNMENT, "A and B must be 16-byte aligned");
-  if ((K * es) % 16 != 0)
+  if ((K * in_es) % 16 != 0)
     return fail(GMM_ERR_ALIGNMENT, "dim * element size must be a multiple of 16 bytes, got dim=" +
                                        std::to_string(K));
   const size_t need = pl.table_bytes;
@@ -1338,6 +1448,11 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
   prm.act = act;
   prm.act_cols = act ? static_cast<int>(N_out) : 0;
   prm.tile_rows = static_cast<int>(tile_rows);
+  if (q) {
+    prm.scale_a = q->a;
+    prm.scale_b = q->b;
+    prm.scale_cols = N;
+  }
   if (inject) {
     prm.drop_kb1 = inject->drop_k_block + 1;
     prm.wait_ns = inject->wait_ns;
@@ -1353,6 +1468,13 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
     prm.inline_ints = static_cast<int>(pl.table.size());
     prm.ext_table = nullptr;
   } else {
+    if (q) {  // a captured copy would read this call's table after it is gone
+      cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+      if ((ce = cudaStreamIsCapturing(stream, &cap)) != cudaSuccess) return cuda_fail(ce, "cudaStreamIsCapturing");
+      if (cap != cudaStreamCaptureStatusNone)
+        return fail(GMM_ERR_INVALID_ARGUMENT,
+                    "more than 1024 non-empty experts cannot be captured into a graph (their table is copied from the host)");
+    }
     ce = cudaMemcpyAsync(workspace, pl.table.data(), pl.table.size() * sizeof(int32_t), cudaMemcpyHostToDevice,
                          stream);
     if (ce != cudaSuccess) return cuda_fail(ce, "cudaMemcpyAsync(table)");
@@ -1360,7 +1482,7 @@ int launch_impl(const PlanObj& po, const Plan& pl, const void* A, const void* B,
   }
 
   return setup_and_launch(prm, A, B, T, K, N, E, dtype, trans_b, tile_rows, act, pl.total_tiles, di, stream,
-                          kind == kTileSwap);
+                          kind == kTileSwap, po.i8);
 }
 
 int forward_impl(const void* A, const void* B, const int64_t* batch_sizes, int64_t num_experts,
@@ -1376,7 +1498,108 @@ int forward_impl(const void* A, const void* B, const int64_t* batch_sizes, int64
   return launch_impl(po, po.pl, A, B, D, workspace, workspace_bytes, stream_ptr, ep, act);
 }
 
+// Grouped GEMM with device-resident batch sizes; q: the scales of 8-bit
+// operands (dtype is then the output type), null for floating-point ones.
+int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_dev, int64_t num_experts,
+                     int64_t rows_cap, int64_t dim, int64_t dim_out, int dtype, int trans_b, int swiglu, void* D,
+                     void* stream_ptr, const I8Scales* q) {
+  NvtxRange range("gmm_sm100 forward_dev");
+  const bool i8 = q != nullptr;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (num_experts < 1 || num_experts > kMaxDevExperts || rows_cap < 0 || dim < 0 || dim_out < 0)
+    return fail(GMM_ERR_INVALID_ARGUMENT, "device batch sizes need 1 <= num_experts <= 1024");
+  if (dtype != GMM_DTYPE_F32 && dtype != GMM_DTYPE_BF16 && dtype != GMM_DTYPE_F16)
+    return fail(GMM_ERR_DTYPE, "Unsupported dtype: only FP32 / BF16 / FP16 are supported");
+  if (swiglu && (dtype == GMM_DTYPE_F32 || dim_out % 16 != 0))
+    return fail(GMM_ERR_INVALID_ARGUMENT, "SwiGLU takes bf16 / fp16 and dim_out a multiple of 16");
+  if (rows_cap > INT32_MAX - 256 || dim > INT32_MAX || dim_out > INT32_MAX)
+    return fail(GMM_ERR_TOO_LARGE, "a dimension exceeds the int32 coordinate range");
+  if (i8 && dim > kMaxI8Dim)
+    return fail(GMM_ERR_TOO_LARGE, "8-bit operands take dim <= 131071 (the sums are 32-bit integers)");
+  const int64_t T = rows_cap, K = dim, N = dim_out, E = num_experts;
+  if (T == 0 || N == 0) return GMM_OK;
+  const int es = elem_size(dtype);   // of D
+  const int in_es = i8 ? 1 : es;     // of A and B
+  const int64_t N_out = swiglu ? N / 2 : N;
+  if (!D || !aligned16(D)) return fail(GMM_ERR_ALIGNMENT, "D must be non-null and 16-byte aligned");
+  if (!batch_sizes_dev || (reinterpret_cast<uintptr_t>(batch_sizes_dev) & 3u))
+    return fail(GMM_ERR_ALIGNMENT, "batch_sizes must be a 4-byte aligned device pointer");
+  if ((N * es) % 16 != 0) return fail(GMM_ERR_ALIGNMENT, "dim_out * element size must be a multiple of 16 bytes");
+  if (i8)
+    if (int src = check_scales(*q)) return src;
+  int dev = 0;
+  cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  DeviceInfo* di = nullptr;
+  int rc = device_info(dev, &di);
+  if (rc != GMM_OK) return rc;
+  if (K == 0) {
+    ce = cudaMemsetAsync(D, 0, static_cast<size_t>(T) * N_out * es, stream);
+    return ce == cudaSuccess ? GMM_OK : cuda_fail(ce, "cudaMemsetAsync");
+  }
+  if (!A || !B || !aligned16(A) || !aligned16(B))
+    return fail(GMM_ERR_ALIGNMENT, "A and B must be non-null and 16-byte aligned");
+  if ((K * in_es) % 16 != 0) return fail(GMM_ERR_ALIGNMENT, "dim * element size must be a multiple of 16 bytes");
+  // Tile kind from the capacity alone (the sizes are only known on the device):
+  // CTA pairs when the capacity averages at least 384 rows per expert,
+  // swap-AB tiles when it averages at most 16 (decode), else 128-row tiles.
+  int64_t tile_rows = 128;
+  bool swap = false;
+  if (dtype != GMM_DTYPE_F32 || i8) {
+    const int force = tile_force();
+    if (force == GMM_TILE_PAIR) tile_rows = 256;
+    else if (force == GMM_TILE_SWAP) swap = !swiglu && !i8;
+    else if (force != GMM_TILE_128) {
+      if (T >= 384 * E) tile_rows = 256;
+      else swap = !swiglu && !i8 && T <= 16 * E;
+    }
+  }
+  const int64_t BN = dtype == GMM_DTYPE_F32 && !i8 ? 128 : 256;
+  const int64_t BK = i8 ? 128 : (dtype == GMM_DTYPE_F32 ? 32 : 64);
+  GmmParams prm;
+  std::memset(&prm, 0, sizeof(prm));
+  prm.d = D;
+  prm.ldd = N_out;
+  prm.n_tiles = static_cast<int>((N + BN - 1) / BN);
+  prm.k_blocks = static_cast<int>((K + BK - 1) / BK);
+  prm.dim_out = static_cast<int>(N_out);
+  prm.act = swiglu ? 1 : 0;
+  prm.act_cols = swiglu ? static_cast<int>(N_out) : 0;
+  prm.dev_bs = batch_sizes_dev;
+  prm.dev_experts = static_cast<int>(E);
+  prm.rows_cap = static_cast<int>(T);
+  prm.tile_rows = static_cast<int>(tile_rows);
+  if (i8) {
+    prm.scale_a = q->a;
+    prm.scale_b = q->b;
+    prm.scale_cols = N;
+  }
+  return setup_and_launch(prm, A, B, T, K, N, E, dtype, trans_b, tile_rows, prm.act, INT32_MAX, di, stream, swap, i8);
+}
+
 }  // namespace
+
+// Shared with the other source files (status.h).
+namespace gmm_sm100 {
+int set_error(int code, const char* msg) noexcept {
+  try {
+    t_last_error = msg;
+  } catch (...) {
+    t_last_error.clear();
+  }
+  return code;
+}
+
+int current_sm_count(int* sms) {
+  int dev = 0;
+  const cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
+  DeviceInfo* di = nullptr;
+  const int rc = device_info(dev, &di);
+  if (rc == GMM_OK) *sms = di->sm_count;
+  return rc;
+}
+}  // namespace gmm_sm100
 
 struct gmm_sm100_plan_s {
   PlanObj po;
@@ -1579,68 +1802,42 @@ size_t gmm_sm100_dev_workspace_size(int64_t num_experts, int64_t rows_cap, int64
 int gmm_sm100_forward_dev(const void* A, const void* B, const int32_t* batch_sizes_dev, int64_t num_experts,
                           int64_t rows_cap, int64_t dim, int64_t dim_out, int dtype, int trans_b, int swiglu,
                           void* D, void* workspace, size_t workspace_bytes, void* stream_ptr) {
-  NvtxRange range("gmm_sm100 forward_dev");
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (num_experts < 1 || num_experts > kMaxDevExperts || rows_cap < 0 || dim < 0 || dim_out < 0)
-    return fail(GMM_ERR_INVALID_ARGUMENT, "device batch sizes need 1 <= num_experts <= 1024");
-  if (dtype != GMM_DTYPE_F32 && dtype != GMM_DTYPE_BF16 && dtype != GMM_DTYPE_F16)
-    return fail(GMM_ERR_DTYPE, "Unsupported dtype: only FP32 / BF16 / FP16 are supported");
-  if (swiglu && (dtype == GMM_DTYPE_F32 || dim_out % 16 != 0))
-    return fail(GMM_ERR_INVALID_ARGUMENT, "SwiGLU takes bf16 / fp16 and dim_out a multiple of 16");
-  if (rows_cap > INT32_MAX - 256 || dim > INT32_MAX || dim_out > INT32_MAX)
-    return fail(GMM_ERR_TOO_LARGE, "a dimension exceeds the int32 coordinate range");
-  const int64_t T = rows_cap, K = dim, N = dim_out, E = num_experts;
-  if (T == 0 || N == 0) return GMM_OK;
-  const int es = elem_size(dtype);
-  const int64_t N_out = swiglu ? N / 2 : N;
-  if (!D || !aligned16(D)) return fail(GMM_ERR_ALIGNMENT, "D must be non-null and 16-byte aligned");
-  if (!batch_sizes_dev || (reinterpret_cast<uintptr_t>(batch_sizes_dev) & 3u))
-    return fail(GMM_ERR_ALIGNMENT, "batch_sizes must be a 4-byte aligned device pointer");
-  if ((N * es) % 16 != 0) return fail(GMM_ERR_ALIGNMENT, "dim_out * element size must be a multiple of 16 bytes");
-  int dev = 0;
-  cudaError_t ce = cudaGetDevice(&dev);
-  if (ce != cudaSuccess) return cuda_fail(ce, "cudaGetDevice");
-  DeviceInfo* di = nullptr;
-  int rc = device_info(dev, &di);
-  if (rc != GMM_OK) return rc;
-  if (K == 0) {
-    ce = cudaMemsetAsync(D, 0, static_cast<size_t>(T) * N_out * es, stream);
-    return ce == cudaSuccess ? GMM_OK : cuda_fail(ce, "cudaMemsetAsync");
-  }
-  if (!A || !B || !aligned16(A) || !aligned16(B))
-    return fail(GMM_ERR_ALIGNMENT, "A and B must be non-null and 16-byte aligned");
-  if ((K * es) % 16 != 0) return fail(GMM_ERR_ALIGNMENT, "dim * element size must be a multiple of 16 bytes");
   (void)workspace, (void)workspace_bytes;  // none needed (gmm_sm100_dev_workspace_size is 0)
-  // Tile kind from the capacity alone (the sizes are only known on the device):
-  // CTA pairs when the capacity averages at least 384 rows per expert,
-  // swap-AB tiles when it averages at most 16 (decode), else 128-row tiles.
-  int64_t tile_rows = 128;
-  bool swap = false;
-  if (dtype != GMM_DTYPE_F32) {
-    const int force = tile_force();
-    if (force == GMM_TILE_PAIR) tile_rows = 256;
-    else if (force == GMM_TILE_SWAP) swap = !swiglu;
-    else if (force != GMM_TILE_128) {
-      if (T >= 384 * E) tile_rows = 256;
-      else swap = !swiglu && T <= 16 * E;
-    }
-  }
-  const int64_t BN = dtype == GMM_DTYPE_F32 ? 128 : 256;
-  const int64_t BK = dtype == GMM_DTYPE_F32 ? 32 : 64;
-  GmmParams prm;
-  std::memset(&prm, 0, sizeof(prm));
-  prm.d = D;
-  prm.ldd = N_out;
-  prm.n_tiles = static_cast<int>((N + BN - 1) / BN);
-  prm.k_blocks = static_cast<int>((K + BK - 1) / BK);
-  prm.dim_out = static_cast<int>(N_out);
-  prm.act = swiglu ? 1 : 0;
-  prm.act_cols = swiglu ? static_cast<int>(N_out) : 0;
-  prm.dev_bs = batch_sizes_dev;
-  prm.dev_experts = static_cast<int>(E);
-  prm.rows_cap = static_cast<int>(T);
-  prm.tile_rows = static_cast<int>(tile_rows);
-  return setup_and_launch(prm, A, B, T, K, N, E, dtype, trans_b, tile_rows, prm.act, INT32_MAX, di, stream, swap);
+  return forward_dev_impl(A, B, batch_sizes_dev, num_experts, rows_cap, dim, dim_out, dtype, trans_b, swiglu, D,
+                          stream_ptr, nullptr);
+}
+
+size_t gmm_sm100_int8_workspace_size(const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens,
+                                     int64_t dim, int64_t dim_out) try {
+  Plan pl;
+  if (make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, GMM_DTYPE_BF16, pl, 128, true) != GMM_OK) return 0;
+  return pl.table_bytes;
+} catch (const std::exception&) {
+  return 0;
+}
+
+int gmm_sm100_forward_int8(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
+                           const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens, int64_t dim,
+                           int64_t dim_out, int out_dtype, int swiglu, void* D, void* workspace,
+                           size_t workspace_bytes, void* stream) try {
+  const int act = swiglu ? 1 : 0;
+  const I8Scales q{scale_a, scale_b};
+  PlanObj po;
+  const int rc = plan_impl(batch_sizes, num_experts, num_tokens, dim, dim_out, out_dtype, 1, act, false, po, true);
+  if (rc != GMM_OK) return rc;
+  return launch_impl(po, po.pl, A, B, D, workspace, workspace_bytes, stream, nullptr, act, nullptr, &q);
+} catch (const std::exception&) {
+  return set_error(GMM_ERR_TOO_LARGE, "host allocation failed");
+}
+
+int gmm_sm100_forward_int8_dev(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
+                               const int32_t* batch_sizes_dev, int64_t num_experts, int64_t rows_cap, int64_t dim,
+                               int64_t dim_out, int out_dtype, int swiglu, void* D, void* stream) try {
+  const I8Scales q{scale_a, scale_b};
+  return forward_dev_impl(A, B, batch_sizes_dev, num_experts, rows_cap, dim, dim_out, out_dtype, 1, swiglu ? 1 : 0, D,
+                          stream, &q);
+} catch (const std::exception&) {
+  return set_error(GMM_ERR_TOO_LARGE, "host allocation failed");
 }
 
 int gmm_sm100_forward_vark(const void* A, const void* B, const int64_t* batch_sizes, int64_t num_experts,
@@ -1709,10 +1906,10 @@ int gmm_sm100_forward_vark(const void* A, const void* B, const int64_t* batch_si
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(total, di->sm_count)));
   const int bit = dtype == GMM_DTYPE_BF16 ? 9 : 10;
   auto launch = [&](auto kern, int smem) -> int {
-    if (!(di->smem_attr_set.load() & (1u << bit))) {
+    if (!(di->smem_attr_set.load() & (1ull << bit))) {
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(vark)");
-      di->smem_attr_set.fetch_or(1u << bit);
+      di->smem_attr_set.fetch_or(1ull << bit);
     }
     kern<<<grid, kThreads, smem, stream>>>(prm);
     cudaError_t e = cudaGetLastError();

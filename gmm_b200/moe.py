@@ -9,7 +9,9 @@
 4. the weighted combine back into token order,
 
 as seven kernel launches with no host synchronisation, so the layer can be
-captured in a CUDA graph.  The reference only provides step 3's grouped GEMM
+captured in a CUDA graph.  ``moe_forward_int8`` is the same layer on 8-bit
+weights and activations, and ``moe_block`` puts the norms, the gate and the
+residual around either.  The reference only provides step 3's grouped GEMM
 (with host ``batch_sizes``); its benchmark leaves routing and gather/scatter
 out (reference ``tests/bench_moe_forward.py:216-217``).
 """
@@ -21,6 +23,8 @@ from typing import Optional, Tuple
 import torch
 
 from gmm_b200 import capi
+from gmm_b200.int8 import gmm_int8, gmm_int8_dev, quantize_rows
+from gmm_b200.norms import post_norm
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -46,30 +50,35 @@ def topk_route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Tuple[
     return ids, w
 
 
-def permute(x: torch.Tensor, ids: torch.Tensor, num_experts: int):
+def permute(x: Optional[torch.Tensor], ids: torch.Tensor, num_experts: int):
     """Token rows in expert order.
 
     Returns ``(x_perm [T*k, dim], batch_sizes int32 [E], dst_pos int32 [T, k],
-    src_token int32 [T*k])``; all stay on the device."""
+    src_token int32 [T*k])``; all stay on the device.  With ``x = None`` only
+    the positions are worked out and ``x_perm`` is ``None``."""
     if ids.dtype != torch.int32 or ids.dim() != 2 or not ids.is_cuda:
         raise ValueError("ids must be a 2D CUDA int32 tensor [T, k]")
-    x = x.contiguous()
     T, k = ids.shape
-    if x.shape[0] != T:
-        raise ValueError("x and ids must have the same number of tokens")
-    dev = x.device
+    dev = ids.device
     n = T * k
-    x_perm = torch.empty(n, x.shape[1], dtype=x.dtype, device=dev)
+    x_perm, row_bytes = None, 0
+    if x is not None:
+        x = x.contiguous()
+        if x.shape[0] != T:
+            raise ValueError("x and ids must have the same number of tokens")
+        x_perm = torch.empty(n, x.shape[1], dtype=x.dtype, device=x.device)
+        row_bytes = x.shape[1] * x.element_size()
     bs = torch.empty(num_experts, dtype=torch.int32, device=dev)
     dst_pos = torch.empty(T, k, dtype=torch.int32, device=dev)
     src_token = torch.empty(n, dtype=torch.int32, device=dev)
     lib = capi.load()
     need = int(lib.gmm_sm100_moe_permute_workspace_size(n, num_experts))
     ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-    _check_moe(lib.gmm_sm100_moe_permute(x.data_ptr(), T, x.shape[1] * x.element_size(),
-                                         ids.contiguous().data_ptr(), k, num_experts, x_perm.data_ptr(),
+    _check_moe(lib.gmm_sm100_moe_permute(None if x is None else x.data_ptr(), T, row_bytes,
+                                         ids.contiguous().data_ptr(), k, num_experts,
+                                         None if x is None else x_perm.data_ptr(),
                                          bs.data_ptr(), dst_pos.data_ptr(), src_token.data_ptr(),
-                                         ws.data_ptr(), need, _stream(x)))
+                                         ws.data_ptr(), need, _stream(ids)))
     return x_perm, bs, dst_pos, src_token
 
 
@@ -119,3 +128,50 @@ def moe_forward(x: torch.Tensor, router_logits: torch.Tensor, w_gate_up: torch.T
     h = grouped_gemm_dev(xp, w_gate_up, bs, trans_gate_up, swiglu=True)
     y = grouped_gemm_dev(h, w_down, bs, trans_down)
     return unpermute(y, dst_pos, w)
+
+
+def moe_ffn_int8(a: torch.Tensor, w_gate_up: Tuple[torch.Tensor, torch.Tensor],
+                 w_down: Tuple[torch.Tensor, torch.Tensor], batch_sizes: torch.Tensor) -> torch.Tensor:
+    """``moe_ffn`` on 8-bit operands: expert-grouped rows ``a``, host ``batch_sizes``.
+
+    The weights are ``quantize_experts`` pairs; activations are quantised row by
+    row before each product, the hidden rows and the result have ``a``'s dtype
+    (bf16 / fp16)."""
+    q, scale = quantize_rows(a)
+    h = gmm_int8(q, scale, *w_gate_up, batch_sizes, out_dtype=a.dtype, swiglu=True)
+    q, scale = quantize_rows(h)
+    return gmm_int8(q, scale, *w_down, batch_sizes, out_dtype=a.dtype)
+
+
+def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_gate_up: Tuple[torch.Tensor, torch.Tensor],
+                     w_down: Tuple[torch.Tensor, torch.Tensor], k: int, renormalize: bool = True) -> torch.Tensor:
+    """``moe_forward`` on 8-bit operands (``quantize_experts`` pairs for the weights).
+
+    Each token is quantised once, straight into the rows of its ``k`` experts;
+    ``x`` is bf16 / fp16.  No host synchronisation."""
+    E = w_gate_up[0].shape[0]
+    ids, w = topk_route(router_logits, k, renormalize)
+    _, bs, dst_pos, _ = permute(None, ids, E)
+    q, scale = quantize_rows(x, dst_pos)
+    h = gmm_int8_dev(q, scale, *w_gate_up, bs, out_dtype=x.dtype, swiglu=True)
+    q, scale = quantize_rows(h)
+    y = gmm_int8_dev(q, scale, *w_down, bs, out_dtype=x.dtype)
+    return unpermute(y, dst_pos, w)
+
+
+def moe_block(x: torch.Tensor, h: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, k: int,
+              post_weight: torch.Tensor, next_weight: Optional[torch.Tensor] = None,
+              gate: Optional[torch.Tensor] = None, gate_act: str = "none", residual_scale: float = 1.0,
+              eps: float = 1e-6, weight_offset: float = 0.0, renormalize: bool = True):
+    """One MoE block of a serving model with norms around it.
+
+    ``x [T, dim]`` is the residual stream and ``h`` its pre-norm (``pre_norm``
+    for the first block, the second result of the previous ``moe_block``
+    after that).  The router's logits are ``h @ w_router`` (``[dim, E]``); the
+    expert weights are tensors (``moe_forward``) or ``quantize_experts`` pairs
+    (``moe_forward_int8``).  Returns what :func:`gmm_b200.norms.post_norm` does:
+    the new residual stream, and with ``next_weight`` the next block's ``h``."""
+    layer = moe_forward_int8 if isinstance(w_gate_up, tuple) else moe_forward
+    y = layer(h, torch.matmul(h, w_router), w_gate_up, w_down, k, renormalize=renormalize)
+    return post_norm(y, x, post_weight, gate=gate, gate_act=gate_act, residual_scale=residual_scale,
+                     next_weight=next_weight, eps=eps, weight_offset=weight_offset)

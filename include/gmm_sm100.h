@@ -192,6 +192,84 @@ int gmm_sm100_moe_unpermute(const void* y, const int32_t* dst_pos, const float* 
                             int64_t num_tokens, int k, int64_t dim_out, int dtype, void* out,
                             void* stream);
 
+/* ------------------------------------------------ 8-bit grouped product
+ * No reference counterpart (the reference multiplies fp32 / bf16 / fp16 only).
+ * Signed 8-bit operands with one fp32 scale for each row of A (token) and
+ * one for each expert and output column (channel):
+ *   D[i][n] = scale_a[i] * scale_b[e][n] * sum_k A[i][k] * B[e][n][k]
+ * A is [num_tokens, dim], B [num_experts, dim_out, dim] (both K-major, dim a
+ * multiple of 16, dim <= 131071), scale_a [num_tokens], scale_b
+ * [num_experts, dim_out].  The sums are exact 32-bit integers; the scaled
+ * result is fp32, rounded once to out_dtype (fp32, bf16 or fp16).  swiglu: B
+ * holds [gate rows | up rows], D is [num_tokens, dim_out / 2] and holds
+ * silu(gate) * up of the scaled sums (bf16 / fp16).  Batch sizes, workspace,
+ * streams and errors as in gmm_sm100_forward / gmm_sm100_forward_dev; A
+ * scale that is NaN makes its row (column) NaN. */
+int gmm_sm100_forward_int8(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
+                           const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens, int64_t dim,
+                           int64_t dim_out, int out_dtype, int swiglu, void* D, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace gmm_sm100_forward_int8 needs: the tile table when
+ * more than 1024 experts are non-empty, else 0. */
+size_t gmm_sm100_int8_workspace_size(const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens,
+                                     int64_t dim, int64_t dim_out);
+
+/* The same with int32 batch sizes in device memory (see gmm_sm100_forward_dev). */
+int gmm_sm100_forward_int8_dev(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
+                               const int32_t* batch_sizes_dev, int64_t num_experts, int64_t rows_cap, int64_t dim,
+                               int64_t dim_out, int out_dtype, int swiglu, void* D, void* stream);
+
+/* Rows to 8-bit codes and a scale each:
+ *   scale = max|x| / 127, code = rint(x / scale)   (both divisions in fp32, correctly rounded)
+ * x is [num_rows, dim] (fp32, bf16 or fp16; dim <= 65536); row t goes to rows
+ * dst_pos[t*k + j], j < k, of q [out_rows, round_up(dim, 16)] (columns past dim
+ * are 0) and of scale [out_rows]; positions outside [0, out_rows) are skipped
+ * (so the dst_pos of gmm_sm100_moe_permute puts the rows into expert order).
+ * dst_pos may be NULL with k = 1: row t to row t.  A row of zeros has scale 0;
+ * a row holding an infinity or a NaN has scale NaN and codes 0.  Two slots
+ * with the same position leave that row undefined unless their rows agree. */
+int gmm_sm100_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t dim, const int32_t* dst_pos,
+                            int k, int64_t out_rows, int8_t* q, float* scale, void* stream);
+
+/* ------------------------------------------------ norms around a block
+ * No reference counterpart.  RMS norm after a block, with the block's gate,
+ * residual scale and residual add, and the next block's RMS norm, in one pass:
+ *   x_new = x + residual_scale * act(gate) * (weight + weight_offset) * y * r(y)
+ *   h     = (next_weight + weight_offset) * x_new * r(x_new)
+ *   r(z)  = 1 / sqrt(mean(z^2) + eps) over the row
+ * y, x, x_new, h are [rows, dim] of dtype (dim <= 16384); weight and
+ * next_weight [dim] of weight_dtype, gate of gate_dtype (each the rows' type
+ * or fp32).  h uses x_new before it is rounded to dtype.  h may be NULL (no
+ * next norm); y may be NULL: then h is the norm of x alone and x_new, weight
+ * and gate are not used.  rstd_y / rstd_x (fp32 [rows], may be NULL) keep
+ * r(y) and r(x_new) for the backward pass. */
+enum gmm_gate_mode {
+  GMM_GATE_MODE_NONE = 0,    /* act(gate) = 1 */
+  GMM_GATE_MODE_CHANNEL = 1, /* gate [dim] */
+  GMM_GATE_MODE_TOKEN = 2,   /* gate [rows] */
+  GMM_GATE_MODE_FULL = 3     /* gate [rows, dim] */
+};
+enum gmm_gate_act { GMM_GATE_IDENTITY = 0, GMM_GATE_TANH = 1, GMM_GATE_SIGMOID = 2 };
+int gmm_sm100_post_norm(const void* y, const void* x, const void* weight, const void* gate, const void* next_weight,
+                        int64_t rows, int64_t dim, int dtype, int weight_dtype, int gate_dtype, int gate_mode,
+                        int gate_act, float residual_scale, float eps, float weight_offset, void* x_new, void* h,
+                        float* rstd_y, float* rstd_x, void* stream);
+
+/* Its gradients, from dx_new and dh (either may be NULL, not both; dh NULL
+ * leaves dnext_weight unwritten).  dy and dx are [rows, dim] of dtype; dweight,
+ * dnext_weight and dgate have the types and shapes of weight, next_weight and
+ * gate, summed in fp32 in a fixed order.  y NULL as in gmm_sm100_post_norm. */
+int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weight, const void* gate,
+                                 const void* next_weight, const float* rstd_y, const float* rstd_x,
+                                 const void* dx_new, const void* dh, int64_t rows, int64_t dim, int dtype,
+                                 int weight_dtype, int gate_dtype, int gate_mode, int gate_act, float residual_scale,
+                                 float weight_offset, void* dy, void* dx, void* dweight, void* dgate,
+                                 void* dnext_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of gmm_sm100_post_norm_backward on the current device. */
+size_t gmm_sm100_post_norm_backward_workspace_size(int64_t rows, int64_t dim);
+
 /* Detail of the last failure of a gmm_sm100_moe_* call on this thread. */
 const char* gmm_sm100_moe_last_error(void);
 
