@@ -54,7 +54,8 @@ struct PairCfg {
   static constexpr uint32_t kIdescHalf = kind_idesc<kKind>(kBMnMajor, BM / 2, BN);
   static constexpr int kHalfABytes = kABytes / 2;  // 64 A rows per CTA in a half tile
   static constexpr int kBarBytes = 256;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes + 1024;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes +
+                                    (is_i8(kKind) ? kScaleBytes : 0) + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -236,36 +237,39 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_pair_kernel(const __grid_cons
     using OutT = KindOut<kKind>;
     const int quarter = warp & 3;
     const uint32_t stage = smem_u32(epi_stage) + quarter * (32 * 128);
+    [[maybe_unused]] float* scale_area =
+        reinterpret_cast<float*>(epi_stage + kEpiStageBytes + kDevTableBytes) + quarter * 256;  // 8-bit kinds
     const uint32_t tempty_leader0 = map_shared_to_rank(smem_u32(tempty_bar), 0);
     int g = 0;
     int local = 0;
     for (int tile = pair; tile < total_tiles; tile += num_pairs, ++local) {
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
+      const Tile t = decode_tile<C::BM, C::BN>(tv, n_tiles, tile, g);
+      // half tile: this CTA holds rows [64 cta, 64 cta + 64) of the tile; warp
+      // q drains rows 32 (q & 1) .. +31 of output columns 128 (q >> 1) .. +127
+      const bool half = halves && t.rows <= C::BM_CTA;
+      const int first = half ? (C::BM_CTA / 2) * static_cast<int>(cta) + (quarter & 1) * 32
+                             : C::BM_CTA * static_cast<int>(cta) + quarter * 32;  // row of the tile
+      const int rows = min(32, half ? min(t.rows - first, C::BM_CTA / 2 - (quarter & 1) * 32) : t.rows - first);
+      const int row0 = t.row0 + first;
+      typename std::conditional<is_i8(kKind), TileScales, int>::type scales;
+      if constexpr (is_i8(kKind)) scales = fetch_scales(p, t.expert, t.n0, row0 + lane, lane < rows, lane);
       if (!mbar_wait(smem_u32(tfull_bar + acc), acc_phase, abort_flag, wait_ns)) break;
       tc_fence_after();
-      const Tile t = decode_tile<C::BM, C::BN>(tv, n_tiles, tile, g);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::BN;
-      if (halves && t.rows <= C::BM_CTA) {
-        // half tile: this CTA holds rows [64 cta, 64 cta + 64) of the tile;
-        // warp q drains rows 32 (q & 1) .. +31 of output columns 128 (q >> 1) .. +127
-        const int rows_cta = t.rows - (C::BM_CTA / 2) * static_cast<int>(cta);
-        const int rb = (quarter & 1) * 32;
-        if (rb < rows_cta)  // warp-uniform
-          drain_slab<OutT, C::BN / 2, is_i8(kKind)>(p, tv, g, t.row0 + (C::BM_CTA / 2) * static_cast<int>(cta) + rb,
-                                      min(32, rows_cta - rb), t.n0 + (quarter >> 1) * (C::BN / 2), taddr,
-                                      stage, lane);
-      } else {
-        const int rows_cta = t.rows - C::BM_CTA * static_cast<int>(cta);
-        const int row0 = t.row0 + C::BM_CTA * static_cast<int>(cta);
-        if (quarter * 32 < rows_cta) {  // warp-uniform
-          const int slab0 = row0 + quarter * 32, rows = min(32, rows_cta - quarter * 32);
-          if (sizeof(OutT) == 2 && p.act) {
-            if constexpr (sizeof(OutT) == 2)
-              drain_slab_swiglu<OutT, is_i8(kKind)>(p, tv, g, slab0, rows, t.n0 >> 1, taddr, stage, lane);
-          } else {
-            drain_slab<OutT, C::BN, is_i8(kKind)>(p, tv, g, slab0, rows, t.n0, taddr, stage, lane);
-          }
+      if (rows > 0) {  // warp-uniform
+        typename std::conditional<is_i8(kKind), AccScaled, AccBits>::type conv;
+        if constexpr (is_i8(kKind))
+          conv = place_scales(scales, scale_area, half ? (quarter >> 1) * (C::BN / 2) : 0, lane);
+        if (half) {
+          drain_slab<OutT, C::BN / 2>(p, tv, g, row0, rows, t.n0 + (quarter >> 1) * (C::BN / 2), taddr, stage, lane,
+                                      conv);
+        } else if (sizeof(OutT) == 2 && p.act) {
+          if constexpr (sizeof(OutT) == 2)
+            drain_slab_swiglu<OutT>(p, tv, g, row0, rows, t.n0 >> 1, taddr, stage, lane, conv);
+        } else {
+          drain_slab<OutT, C::BN>(p, tv, g, row0, rows, t.n0, taddr, stage, lane, conv);
         }
       }
       tc_fence_before();

@@ -63,6 +63,7 @@ static_assert((3 * kMaxDevExperts + 6) % 2 == 0 && (3 * kMaxDevExperts + 6) * 4 
 constexpr int kMBlock = 16;          // m-tiles per raster block (L2 reuse of B columns)
 constexpr int kThreads = 256;        // 8 warps: TMA, MMA, TMEM alloc, idle, 4x epilogue
 constexpr int kEpiStageBytes = 4 * 32 * 128;  // epilogue staging: 4 warps x 32 rows x 128 B
+constexpr int kScaleBytes = 4 * 256 * 4;      // 8-bit kinds: 4 warps x the scales of 256 accumulator columns
 
 struct __align__(64) GmmParamsBase {
   CUtensorMap tmap_a;   // A (fp32: raw fp32 tiles, split into TF32 hi/lo in shared memory)
@@ -164,7 +165,8 @@ struct Cfg {
   static constexpr int kTmemCols = 2 * BN;  // double-buffered fp32 accumulator
   static constexpr uint32_t kIdesc = kind_idesc<kKind>(kBMnMajor, BM, BN);
   static constexpr int kBarBytes = 256;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes + 1024;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kEpiStageBytes + kDevTableBytes +
+                                    (is_i8(kKind) ? kScaleBytes : 0) + 1024;
   static_assert(kABytes % 1024 == 0 && kBBytes % 1024 == 0, "swizzle atoms need 1 KB alignment");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
@@ -348,29 +350,27 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 
 // How an accumulator word becomes a number.  Floating-point kinds: its bits.
 struct AccBits {
-  __device__ __forceinline__ void load(int, int) {}
+  __device__ __forceinline__ void load(int) {}
   __device__ __forceinline__ float get(uint32_t v, int) const { return __uint_as_float(v); }
 };
 // 8-bit kinds: the integer sum times its row's and its column's scale.  The
 // sum (below 2^31) rounds to 24 bits once, and the products once each, so the
 // result is within 3 half-steps of fp32 before the one rounding to the output
-// type.  Every lane of a warp works on the same 32 columns, so load() fetches
-// their scales as eight uniform 16-byte loads; columns from `end` on (past
-// dim_out, a multiple of 4) are not read.
+// type.  The column scales of a tile sit in shared memory by accumulator
+// column (fetch_scales), read as uniform 16-byte loads.
 struct AccScaled {
   float row;
-  const float* col;  // scales of the expert's columns
+  const float* col;
   float c[32];
-  __device__ __forceinline__ void load(int c0, int end) {
+  __device__ __forceinline__ void load(int col0) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (c0 + 4 * q < end) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(col + c0 + 4 * q));
-        c[4 * q] = f.x;
-        c[4 * q + 1] = f.y;
-        c[4 * q + 2] = f.z;
-        c[4 * q + 3] = f.w;
-      }
+    for (int q = 0; q < 8; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(col + col0 + 4 * q);
+      c[4 * q] = f.x;
+      c[4 * q + 1] = f.y;
+      c[4 * q + 2] = f.z;
+      c[4 * q + 3] = f.w;
+    }
   }
   __device__ __forceinline__ float get(uint32_t v, int i) const {
     return __int2float_rn(static_cast<int>(v)) * row * c[i];
@@ -387,7 +387,8 @@ struct AccScaled {
 // without reading TMEM (a tile whose contraction is empty).
 template <typename OutT, int BN, typename Acc = AccBits>
 __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim_out, uint32_t taddr,
-                                           uint32_t stage, int lane, bool zero = false, Acc acc = Acc()) {
+                                           uint32_t stage, int lane, bool zero = false,
+                                           Acc acc = Acc()) {
   constexpr int kColsPerSeg = 128 / static_cast<int>(sizeof(OutT));  // 64 (16-bit) or 32 (fp32)
   constexpr int kElemsPer16 = 16 / static_cast<int>(sizeof(OutT));
   const int ch = lane & 7;
@@ -401,7 +402,7 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
       uint32_t v[32];
       if (!zero) {
         tmem_ld_32x32b_x32(taddr + c0 + h * 32, v);
-        acc.load(col + h * 32, dim_out);
+        acc.load(c0 + h * 32);
         tmem_wait_ld();
       } else {
 #pragma unroll
@@ -439,31 +440,56 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
   }
 }
 
-// The scales of a slab: lane l's row is slab_row0 + l.
-__device__ __forceinline__ AccScaled slab_scales(const GmmParamsBase& p, int expert, int slab_row0,
-                                                 int slab_rows, int lane) {
+// The scales one epilogue warp needs for a tile, fetched before it waits for
+// the accumulator: cold reads chunk by chunk during the drain cost more than
+// the rest of it.  One B200, both ways: decode (128 experts, 1..16 rows,
+// 768 x 2048) 61.5 -> 41.1 us; 16384 x 4096 x 14336 on 8 experts 736 -> 633
+// us (3.04 POPS); 4099 rows on 64 experts of 7168 x 4096 331 -> 295 us.
+struct TileScales {
+  float4 c[2];  // accumulator columns 4 * lane .. +3 and 128 + 4 * lane .. +3
+  float row;    // lane's row
+};
+
+// `row`: row of A of this lane, `live`: whether it belongs to the tile.
+__device__ __forceinline__ TileScales fetch_scales(const GmmParamsBase& p, int expert, int n0, int row, bool live,
+                                                   int lane) {
+  TileScales s;
+  const float* col = p.scale_b + expert * p.scale_cols;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // SwiGLU: accumulator columns [0, 128) are gate, [128, 256) up columns
+    const int c = (p.act ? n0 >> 1 : n0 + 128 * i) + 4 * lane;
+    s.c[i] = c < p.dim_out ? __ldg(reinterpret_cast<const float4*>(col + (p.act ? i * p.act_cols : 0) + c))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  s.row = live ? __ldg(p.scale_a + row) : 0.f;
+  return s;
+}
+
+// Into the warp's area; `col0`: first accumulator column the drain counts as 0.
+__device__ __forceinline__ AccScaled place_scales(const TileScales& s, float* area, int col0, int lane) {
+  __syncwarp();  // the previous tile's reads are done
+  reinterpret_cast<float4*>(area)[lane] = s.c[0];
+  reinterpret_cast<float4*>(area)[32 + lane] = s.c[1];
+  __syncwarp();
   AccScaled a;
-  a.row = lane < slab_rows ? __ldg(p.scale_a + slab_row0 + lane) : 0.f;
-  a.col = p.scale_b + expert * p.scale_cols;
+  a.row = s.row;
+  a.col = area + col0;
   return a;
 }
 
 // drain_rows for a slab of grouped-GEMM rows: destinations from out_row().
-template <typename OutT, int BN, bool kI8 = false>
+template <typename OutT, int BN, typename Acc>
 __device__ __forceinline__ void drain_slab(const GmmParamsBase& p, const TableView& tv, int g,
                                            int slab_row0, int slab_rows, int n0, uint32_t taddr,
-                                           uint32_t stage, int lane) {
+                                           uint32_t stage, int lane, const Acc& acc) {
   OutT* rp[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int rr = i * 4 + (lane >> 3);
     rp[i] = rr < slab_rows ? out_row<OutT>(p, tv, g, slab_row0 + rr) : nullptr;
   }
-  if constexpr (kI8)
-    drain_rows<OutT, BN, AccScaled>(rp, n0, p.dim_out, taddr, stage, lane, false,
-                                    slab_scales(p, tv.expert[g], slab_row0, slab_rows, lane));
-  else
-    drain_rows<OutT, BN>(rp, n0, p.dim_out, taddr, stage, lane);
+  drain_rows<OutT, BN, Acc>(rp, n0, p.dim_out, taddr, stage, lane, false, acc);
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
@@ -471,10 +497,10 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 // SwiGLU variant of drain_slab: TMEM columns [0, 128) hold the tile's gate
 // projections and [128, 256) the matching up projections; writes
 // silu(gate) * up (fp32) rounded to the output type, 128 columns per tile.
-template <typename OutT, bool kI8 = false>
+template <typename OutT, typename Acc>
 __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const TableView& tv, int g,
                                                   int slab_row0, int slab_rows, int n0, uint32_t taddr,
-                                                  uint32_t stage, int lane) {
+                                                  uint32_t stage, int lane, const Acc& acc) {
   static_assert(sizeof(OutT) == 2, "SwiGLU epilogue is 16-bit");
   OutT* rp[8];
 #pragma unroll
@@ -482,13 +508,7 @@ __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const 
     const int rr = i * 4 + (lane >> 3);
     rp[i] = rr < slab_rows ? out_row<OutT>(p, tv, g, slab_row0 + rr) : nullptr;
   }
-  using Acc = typename std::conditional<kI8, AccScaled, AccBits>::type;
-  Acc ag, au;  // gate and up
-  if constexpr (kI8) {
-    ag = slab_scales(p, tv.expert[g], slab_row0, slab_rows, lane);
-    au = ag;
-    au.col += p.act_cols;
-  }
+  Acc ag = acc, au = acc;  // gate and up
   const int ch = lane & 7;
   const uint32_t my_row = stage + lane * 128;
 #pragma unroll 1
@@ -500,8 +520,8 @@ __device__ __forceinline__ void drain_slab_swiglu(const GmmParamsBase& p, const 
       uint32_t gv[32], uv[32];
       tmem_ld_32x32b_x32(taddr + c0 + h * 32, gv);
       tmem_ld_32x32b_x32(taddr + 128 + c0 + h * 32, uv);
-      ag.load(col + h * 32, p.dim_out);
-      au.load(col + h * 32, p.dim_out);
+      ag.load(c0 + h * 32);
+      au.load(128 + c0 + h * 32);
       tmem_wait_ld();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -795,22 +815,28 @@ __global__ void __launch_bounds__(kThreads, 1) gmm_persistent_kernel(const __gri
     using OutT = KindOut<kKind>;
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
     const uint32_t stage = smem_u32(epi_stage) + quarter * (32 * 128);
+    [[maybe_unused]] float* scale_area =
+        reinterpret_cast<float*>(epi_stage + kEpiStageBytes + kDevTableBytes) + quarter * 256;  // 8-bit kinds
     int g = 0;
     int local = 0;
     for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
+      const Tile t = decode_tile<C::BM, C::BN>(tv, n_tiles, tile, g);
+      const int row0 = t.row0 + quarter * 32, rows = min(32, t.rows - quarter * 32);
+      typename std::conditional<is_i8(kKind), TileScales, int>::type scales;
+      if constexpr (is_i8(kKind)) scales = fetch_scales(p, t.expert, t.n0, row0 + lane, lane < rows, lane);
       if (!mbar_wait(smem_u32(tfull_bar + acc), acc_phase, abort_flag, wait_ns)) break;
       tc_fence_after();
-      const Tile t = decode_tile<C::BM, C::BN>(tv, n_tiles, tile, g);
-      if (quarter * 32 < t.rows) {  // warp-uniform: some row of this quarter is live
+      if (rows > 0) {  // warp-uniform: some row of this quarter is live
+        typename std::conditional<is_i8(kKind), AccScaled, AccBits>::type conv;
+        if constexpr (is_i8(kKind)) conv = place_scales(scales, scale_area, 0, lane);
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::BN;
-        const int row0 = t.row0 + quarter * 32, rows = min(32, t.rows - quarter * 32);
         if (sizeof(OutT) == 2 && p.act) {
           if constexpr (sizeof(OutT) == 2)
-            drain_slab_swiglu<OutT, is_i8(kKind)>(p, tv, g, row0, rows, t.n0 >> 1, taddr, stage, lane);
+            drain_slab_swiglu<OutT>(p, tv, g, row0, rows, t.n0 >> 1, taddr, stage, lane, conv);
         } else {
-          drain_slab<OutT, C::BN, is_i8(kKind)>(p, tv, g, row0, rows, t.n0, taddr, stage, lane);
+          drain_slab<OutT, C::BN>(p, tv, g, row0, rows, t.n0, taddr, stage, lane, conv);
         }
       }
       tc_fence_before();
