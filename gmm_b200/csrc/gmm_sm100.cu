@@ -1973,7 +1973,9 @@ int gmm_sm100_device_error(int* status_out, int clear) {
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyToSymbol(g_device_error)");
   }
-  if (status_out) *status_out = v;
+  int norm = 0;
+  if (int rc = norm_device_error(&norm, clear != 0)) return rc;
+  if (status_out) *status_out = v ? v : norm;
   return GMM_OK;
 }
 

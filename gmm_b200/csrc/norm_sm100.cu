@@ -23,16 +23,27 @@
 // Everything is held in fp32 and rounded once, on store.  Rows are walked by
 // blocks in a fixed order and parameter gradients added up per block, then
 // over blocks in order, so results do not change from run to run.
+//
+// Bound by HBM: a row is read once and written once.  The kernels stream
+// rows into shared memory with bulk copies (no registers and no threads held
+// by loads in flight), several rows ahead of the two block-wide sums a row
+// waits for; parameters stay in registers over all rows of a block.
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
+#include <type_traits>
 
 #include "gmm_sm100.h"
 #include "row_vec.cuh"
+#include "sm100_ptx.cuh"
 #include "status.h"
 
 namespace gmm_sm100 {
 namespace {
+
+// Set when a wait for a copy ran out (gmm_sm100_device_error reads it).
+__device__ int g_norm_error = 0;
 
 constexpr int kMaxNormDim = 16384;
 constexpr int kMaxThreads = 512;
@@ -54,7 +65,7 @@ struct NormParams {
   void* dgate_row;    // token / full gate gradient
   float* rstd_y;      // [rows], null: not kept
   float* rstd_x;
-  float* partial;     // backward: [3][blocks][D] sums of dw, dv, dgate (channel)
+  float* partial;     // backward: [2][blocks][D], the blocks' sums of act(g) dx yh (1 for a channel gate) and dh xh
   long long rows;
   int dim;
   int w_f32, gate_f32;  // parameters in fp32 (else the rows' type)
@@ -62,19 +73,11 @@ struct NormParams {
   float scale, eps, offset;
 };
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_param(const void* p, int f32, long long at, int col, int dim, float (&f)[8]) {
-  if (f32 || sizeof(T) == 4) {
-    const Raw8<float> r = load8<float, kVec>(static_cast<const float*>(p) + at, col, dim);
-    unpack(r, f);
-  } else {
-    const Raw8<T> r = load8<T, kVec>(static_cast<const T*>(p) + at, col, dim);
-    unpack(r, f);
-  }
-}
-
 __device__ __forceinline__ float act_of(float g, int act) {
-  return act == GMM_GATE_TANH ? tanhf(g) : act == GMM_GATE_SIGMOID ? 1.f / (1.f + expf(-g)) : g;
+  // The sigmoid's fast exponential is within (2 |g| + 4) * 2^-24 of e^-g and
+  // its fast reciprocal within 2 * 2^-24; expf and a full division made a
+  // gate per element cost more than its rows' bytes (8191 x 6144 fp16: 111 us).
+  return act == GMM_GATE_TANH ? tanhf(g) : act == GMM_GATE_SIGMOID ? __fdividef(1.f, 1.f + __expf(-g)) : g;
 }
 // act'(g) from a = act(g)
 __device__ __forceinline__ float act_slope(float a, int act) {
@@ -104,20 +107,7 @@ __device__ __forceinline__ void block_sum(float (&s)[n], float* scratch) {
   }
 }
 
-// The gate of a chunk: act(g) (ones without a gate); `token` is the row's
-// value of a token gate, already through act.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_gate(const NormParams& p, long long row, int col, float token, float (&a)[8]) {
-  if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
-    load_param<T, kVec>(p.gate, p.gate_f32, p.gate_mode == kGateFull ? row * p.dim : 0, col, p.dim, a);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = act_of(a[j], p.act);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = token;
-  }
-}
-
+// act(g) of a token gate's row, 1 for the others.
 template <typename T>
 __device__ __forceinline__ float token_gate(const NormParams& p, long long row) {
   if (p.gate_mode != kGateToken) return 1.f;
@@ -125,180 +115,615 @@ __device__ __forceinline__ float token_gate(const NormParams& p, long long row) 
   return act_of(g, p.act);
 }
 
-// One block per row (grid-stride); a thread holds the 8-element chunks
-// threadIdx.x + i * blockDim.x of the row in registers.
-template <typename T, int kChunks, bool kVec>
-__global__ void __launch_bounds__(kMaxThreads) norm_fwd_kernel(const NormParams p) {
-  __shared__ float scratch[2][32];
-  const int D = p.dim;
-  const float inv_d = 1.f / static_cast<float>(D);
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const T* x = static_cast<const T*>(p.x) + row * D;
-    float xs[kChunks][8];
+// ------------------------------------------------------------------ ring kernels
+// A thread owns kE elements of every row, in units of V neighbouring elements:
+// the units threadIdx.x + i * blockDim.x.  V is 16 bytes where every row
+// starts on a 16-byte boundary, else 1 (neighbouring threads then read
+// neighbouring elements).
+enum RingMode { kPreNorm = 0, kSharedGate = 1, kFullGate = 2 };  // no y | gate none, channel, token | gate per element
+
+template <typename T>
+constexpr int kV = 16 / static_cast<int>(sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& r, float* f) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) unpack(load8<T, kVec>(x, (threadIdx.x + i * blockDim.x) * 8, D), xs[i]);
-    if (p.y) {
-      const T* y = static_cast<const T*>(p.y) + row * D;
-      float ys[kChunks][8];
-      float sq[1] = {0.f};
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = unpack2(w[i], static_cast<const T*>(nullptr));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  } else {
+    f[0] = __uint_as_float(r.x);
+    f[1] = __uint_as_float(r.y);
+    f[2] = __uint_as_float(r.z);
+    f[3] = __uint_as_float(r.w);
+  }
+}
+
+// Unit c of a row of T (shared or global memory), as it lies there and as fp32.
+template <typename T, int V>
+using RawUnit = typename std::conditional<V == 1, T, uint4>::type;
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack_unit(const RawUnit<T, V>& r, float* f) {
+  if constexpr (V == 1) f[0] = as_float(r);
+  else unpack16<T>(r, f);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void read_unit(const void* row, int c, float* f) {
+  unpack_unit<T, V>(static_cast<const RawUnit<T, V>*>(row)[c], f);
+}
+
+// The same, 0 where the unit is past the row's end (`in` false).
+template <typename T, int V>
+__device__ __forceinline__ void read_unit_or_0(const void* row, int c, bool in, float* f) {
+  RawUnit<T, V> r = {};
+  if (in) r = static_cast<const RawUnit<T, V>*>(row)[c];
+  unpack_unit<T, V>(r, f);
+}
+
+// Unit c of a parameter or gate row that is T or fp32.
+template <typename T, int V>
+__device__ __forceinline__ void read_param(const void* row, bool f32, int c, float* f) {
+  if (f32 && sizeof(T) == 2) {
+    if constexpr (V == 1) {
+      f[0] = static_cast<const float*>(row)[c];
+    } else {
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        unpack(load8<T, kVec>(y, (threadIdx.x + i * blockDim.x) * 8, D), ys[i]);
+      for (int q = 0; q < V / 4; ++q) unpack16<float>(static_cast<const uint4*>(row)[c * (V / 4) + q], f + 4 * q);
+    }
+  } else {
+    read_unit<T, V>(row, c, f);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void write_unit(T* row, int c, const float* f) {
+  if constexpr (V == 1) {
+    row[c] = from_float<T>(f[0]);
+  } else if constexpr (sizeof(T) == 2) {
+    const T* t = nullptr;
+    reinterpret_cast<uint4*>(row)[c] = make_uint4(pack_pair(f[0], f[1], t), pack_pair(f[2], f[3], t),
+                                                  pack_pair(f[4], f[5], t), pack_pair(f[6], f[7], t));
+  } else {
+    reinterpret_cast<float4*>(row)[c] = make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Bytes a row takes in a slot: it keeps its offset within 16 bytes there.
+__host__ __device__ constexpr uint32_t row_pitch(uint32_t row_bytes, bool aligned) {
+  return aligned ? row_bytes : (row_bytes + 15 + 15) / 16 * 16;
+}
+
+// A ring of row slots in shared memory, filled by bulk copies, which take
+// whole 16-byte words.  A slot holds one row of each input that is there.
+// kAligned: every row starts and ends on a word; otherwise a row is fetched
+// with the words it shares with its neighbours, except at a tensor's two
+// ends, where those words may reach beyond it: there only whole words come by
+// the copy, and the block's threads bring the bytes around them.
+template <int kInputs, bool kAligned>
+struct RowRing {
+  const char* src[kInputs];
+  uint32_t bytes[kInputs];  // of a row; 0: input not there
+  long long rows;
+  uint8_t* smem;            // slot 0
+  uint32_t slot_bytes;
+  uint32_t bars;            // shared address of the slots' barriers
+  int slots;
+  bool dead;                // a wait ran out: no more waiting or loading, the error word says so
+
+  __device__ __forceinline__ uint32_t pitch(int i) const { return bytes[i] ? row_pitch(bytes[i], kAligned) : 0; }
+
+  // One thread: fetch `row` into `slot`.
+  __device__ __forceinline__ void fetch(int slot, long long row) const {
+    const uint32_t bar = bars + 8 * slot;
+    const bool inner = edge(row);  // only the words that lie wholly inside the row
+    const char* from[kInputs];
+    uint32_t len[kInputs], to[kInputs], total = 0, at = smem_u32(smem) + slot * slot_bytes;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sq[0] = fmaf(ys[i][j], ys[i][j], sq[0]);
+    for (int i = 0; i < kInputs; ++i) {
+      from[i] = src[i] + row * bytes[i];
+      len[i] = bytes[i];
+      to[i] = at;
+      if (!kAligned && bytes[i]) {
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from[i]) & 15u);
+        const uint32_t lo = inner ? (off + 15u) & ~15u : 0u;  // from the first word's start
+        const uint32_t hi = inner ? (off + bytes[i]) & ~15u : (off + bytes[i] + 15u) & ~15u;
+        len[i] = hi > lo ? hi - lo : 0u;
+        from[i] += static_cast<int>(lo) - static_cast<int>(off);
+        to[i] += lo;
       }
-      block_sum(sq, scratch[0]);
+      total += len[i];
+      at += pitch(i);
+    }
+    mbar_arrive_expect_tx(bar, total);
+#pragma unroll
+    for (int i = 0; i < kInputs; ++i)
+      if (len[i]) bulk_load(to[i], from[i], len[i], bar);
+  }
+
+  // Whether the words of `row` may reach beyond an input's first or last byte
+  // (they reach at most 15 bytes past the row on either side).
+  __device__ __forceinline__ bool edge(long long row) const {
+    if (kAligned) return false;
+    long long least = INT64_MAX;
+#pragma unroll
+    for (int i = 0; i < kInputs; ++i)
+      if (bytes[i]) least = min(least, static_cast<long long>(bytes[i]));
+    return row * least < 15 || (rows - 1 - row) * least < 15;
+  }
+
+  // All threads: wait for the row in `slot`.
+  __device__ __forceinline__ void wait(int slot, uint32_t parity, long long row) {
+    if (!dead) {
+      const uint32_t bar = bars + 8 * slot;
+      if (!mbar_try_wait(bar, parity)) {
+        const unsigned long long t0 = global_timer_ns();
+        while (!mbar_try_wait(bar, parity))
+          if (global_timer_ns() - t0 > kWaitTimeoutNs) {
+            dead = true;
+            atomicCAS(&g_norm_error, 0, GMM_ERR_DEVICE_TIMEOUT);
+            break;
+          }
+      }
+    }
+    if (!edge(row)) return;
+    // the row's bytes before its first and after its last whole word, at most
+    // 15 on each side (rows are a multiple of 2 bytes)
+    uint8_t* base = smem + slot * slot_bytes;
+#pragma unroll
+    for (int i = 0; i < kInputs; ++i) {
+      const char* from = src[i] + row * bytes[i];
+      const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 15u);
+      const uint32_t lo = (off + 15u) & ~15u, hi = (off + bytes[i]) & ~15u, end = off + bytes[i];
+      for (uint32_t k = off + 2 * threadIdx.x; k < end; k += 2 * blockDim.x)
+        if (k < lo || k >= hi)
+          *reinterpret_cast<uint16_t*>(base + k) = *reinterpret_cast<const uint16_t*>(from + (k - off));
+      base += pitch(i);
+    }
+    fence_proxy_async_smem();  // the slot's next contents come by a bulk copy
+    __syncthreads();
+  }
+
+  // Input i of the row in `slot`.
+  __device__ __forceinline__ const uint8_t* get(int slot, int i, long long row) const {
+    uint32_t at = slot * slot_bytes;
+#pragma unroll
+    for (int j = 0; j < i; ++j) at += pitch(j);
+    if (!kAligned) at += static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u);
+    return smem + at;
+  }
+
+  // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  The
+  // caller synchronises the block before the first wait.
+  __device__ __forceinline__ void start(uint8_t* mem, int n, long long num_rows) {
+    smem = mem;
+    slots = n;
+    rows = num_rows;
+    dead = false;
+    slot_bytes = 0;
+#pragma unroll
+    for (int i = 0; i < kInputs; ++i) slot_bytes += pitch(i);
+    bars = smem_u32(mem) + slots * slot_bytes;
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < slots; ++s) mbar_init(bars + 8 * s, 1);
+      fence_mbarrier_init();
+      for (int s = 0; s < slots; ++s) {
+        const long long row = blockIdx.x + static_cast<long long>(s) * gridDim.x;
+        if (row < rows) fetch(s, row);
+      }
+    }
+  }
+};
+
+// s (w + o), times act(g) of a channel gate; v + o.  Zero past the row's end.
+template <typename T, int V, int kE, int kMode>
+__device__ __forceinline__ void row_params(const NormParams& p, bool with_v, float (&pw)[kE], float (&vo)[kE]) {
+  const int units = p.dim / V;
+#pragma unroll
+  for (int i = 0; i < kE / V; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) pw[i * V + j] = vo[i * V + j] = 0.f;
+    if (c >= units) continue;
+    if constexpr (kMode != kPreNorm) {
+      read_param<T, V>(p.w, p.w_f32, c, pw + i * V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) pw[i * V + j] = (pw[i * V + j] + p.offset) * p.scale;
+      if (kMode == kSharedGate && p.gate_mode == kGateChannel) {
+        float g[V];
+        read_param<T, V>(p.gate, p.gate_f32, c, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) pw[i * V + j] *= act_of(g[j], p.act);
+      }
+    }
+    if (with_v) {
+      read_param<T, V>(p.v, p.w_f32, c, vo + i * V);
+#pragma unroll
+      for (int j = 0; j < V; ++j) vo[i * V + j] += p.offset;
+    }
+  }
+}
+
+template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const NormParams p, int slots) {
+  constexpr int kUnits = kE / V;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float scratch[2][2][32];  // by sum and by parity of the row
+  const int D = p.dim;
+  RowRing<3, (V > 1)> ring;
+  ring.src[0] = static_cast<const char*>(p.x);
+  ring.src[1] = static_cast<const char*>(p.y);
+  ring.src[2] = static_cast<const char*>(p.gate);
+  ring.bytes[0] = D * sizeof(T);
+  ring.bytes[1] = kMode == kPreNorm ? 0 : D * sizeof(T);
+  ring.bytes[2] = kMode == kFullGate ? D * (p.gate_f32 ? 4 : static_cast<int>(sizeof(T))) : 0;
+  ring.start(smem, slots, p.rows);
+
+  const int units = D / V;
+  float pw[kE], vo[kE];
+  row_params<T, V, kE, kMode>(p, p.h != nullptr, pw, vo);
+  __syncthreads();  // barriers initialised
+  const float inv_d = 1.f / static_cast<float>(D);
+
+  int slot = 0;
+  uint32_t phase = 0;
+  int odd = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
+    ring.wait(slot, phase, row);
+    const auto* xs = reinterpret_cast<const RawUnit<T, V>*>(ring.get(slot, 0, row));
+    float x[kE];
+    float sq[1] = {0.f};
+    if constexpr (kMode == kPreNorm) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
+        read_unit_or_0<T, V>(xs, c, c < units, x + i * V);
+      }
+    } else {
+      const uint8_t* ys = ring.get(slot, 1, row);
+      float y[kE];
+      RawUnit<T, V> xr[kUnits];
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
+        read_unit_or_0<T, V>(ys, c, c < units, y + i * V);
+        xr[i] = RawUnit<T, V>{};
+        if (c < units) xr[i] = xs[c];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sq[0] = fmaf(y[i * V + j], y[i * V + j], sq[0]);
+        if constexpr (kMode == kFullGate) {  // y * act(g): the gate is not needed again
+          float g[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] = 0.f;
+          if (c < units) read_param<T, V>(ring.get(slot, 2, row), p.gate_f32, c, g);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[i * V + j] *= act_of(g[j], p.act);
+        }
+      }
+      block_sum(sq, scratch[0][odd]);
       const float ry = rsqrtf(sq[0] * inv_d + p.eps);
       if (p.rstd_y && threadIdx.x == 0) p.rstd_y[row] = ry;
-      const float tok = token_gate<T>(p, row);
+      const float c0 = ry * tok;
       T* xn = static_cast<T*>(p.xn) + row * D;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        float w[8], a[8];
-        load_param<T, kVec>(p.w, p.w_f32, 0, col, D, w);
-        load_gate<T, kVec>(p, row, col, tok, a);
+      for (int i = 0; i < kUnits; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
+        unpack_unit<T, V>(xr[i], x + i * V);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          xs[i][j] = col + j < D ? fmaf(p.scale * a[j], (w[j] + p.offset) * (ys[i][j] * ry), xs[i][j]) : 0.f;
-        store8<T, kVec>(xn, col, D, xs[i]);
+        for (int j = 0; j < V; ++j)
+          x[i * V + j] = fmaf(y[i * V + j] * c0, pw[i * V + j], x[i * V + j]);
+        if (c < units) write_unit<T, V>(xn, c, x + i * V);
       }
     }
     if (p.h) {
-      float sq[1] = {0.f};
+      sq[0] = 0.f;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sq[0] = fmaf(xs[i][j], xs[i][j], sq[0]);
-      block_sum(sq, scratch[1]);
+      for (int j = 0; j < kE; ++j) sq[0] = fmaf(x[j], x[j], sq[0]);
+      block_sum(sq, scratch[1][odd]);
       const float rx = rsqrtf(sq[0] * inv_d + p.eps);
       if (p.rstd_x && threadIdx.x == 0) p.rstd_x[row] = rx;
       T* h = static_cast<T*>(p.h) + row * D;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int col = (threadIdx.x + i * blockDim.x) * 8;
-        float v[8], o[8];
-        load_param<T, kVec>(p.v, p.w_f32, 0, col, D, v);
+      for (int i = 0; i < kUnits; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (v[j] + p.offset) * (xs[i][j] * rx);
-        store8<T, kVec>(h, col, D, o);
+        for (int j = 0; j < V; ++j) x[i * V + j] *= rx * vo[i * V + j];
+        if (c < units) write_unit<T, V>(h, c, x + i * V);
       }
     }
-    __syncthreads();  // scratch is reused by the next row
+    // Every thread has read the slot before the (first or only) sum's barrier.
+    if (blockDim.x == 32) __syncwarp();
+    if (threadIdx.x == 0 && !ring.dead) {
+      const long long next = row + static_cast<long long>(slots) * gridDim.x;
+      if (next < p.rows) ring.fetch(slot, next);
+    }
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+    odd ^= 1;  // the next row's sums use the other scratch: its barriers free this one
   }
 }
 
-// Backward of the same rows; a block adds up its rows' parameter gradients in
-// registers (a thread owns its columns) and leaves them in `partial`.
-template <typename T, int kChunks, bool kVec>
+// Backward.  The rows stay in the ring between the sums and the results
+// (re-reading shared memory costs less than holding four rows in registers),
+// so a slot is refilled one row later, past the next row's barrier -- or, with
+// a single slot, behind a barrier of its own.
+template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const NormParams p, int slots) {
+  constexpr int kUnits = kE / V;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float scratch[2][3 * 32];
+  const int D = p.dim;
+  RowRing<5, (V > 1)> ring;
+  ring.src[0] = static_cast<const char*>(p.x);
+  ring.src[1] = static_cast<const char*>(p.y);
+  ring.src[2] = static_cast<const char*>(p.dxn);
+  ring.src[3] = static_cast<const char*>(p.dh);
+  ring.src[4] = static_cast<const char*>(p.gate);
+  ring.bytes[0] = D * sizeof(T);
+  ring.bytes[1] = kMode == kPreNorm ? 0 : D * sizeof(T);
+  ring.bytes[2] = p.dxn ? D * sizeof(T) : 0;
+  ring.bytes[3] = p.dh ? D * sizeof(T) : 0;
+  ring.bytes[4] = kMode == kFullGate ? D * (p.gate_f32 ? 4 : static_cast<int>(sizeof(T))) : 0;
+  ring.start(smem, slots, p.rows);
+
+  const int units = D / V;
+  float pw[kE], vo[kE], acc[kE], dv[kE];
+  row_params<T, V, kE, kMode>(p, p.dh != nullptr, pw, vo);
+#pragma unroll
+  for (int j = 0; j < kE; ++j) acc[j] = dv[j] = 0.f;
+  __syncthreads();  // barriers initialised
+  const float inv_d = 1.f / static_cast<float>(D);
+
+  int slot = 0;
+  uint32_t phase = 0;
+  int odd = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float ry = kMode == kPreNorm ? 0.f : p.rstd_y[row];
+    const float rx = p.dh ? p.rstd_x[row] : 0.f;
+    const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
+    ring.wait(slot, phase, row);
+    const uint8_t *in_x = ring.get(slot, 0, row), *in_y = ring.get(slot, 1, row), *in_dx = ring.get(slot, 2, row),
+                  *in_dh = ring.get(slot, 3, row), *in_g = ring.get(slot, 4, row);
+    // yh, e = dx' + rx u, xh, act(g), dh of unit i
+    // (past the row's end: zeros, as its parameters are; a branch around each
+    // unit would keep single elements' loads from being in flight together)
+    auto read = [&](int i, int c, float (&yh)[V], float (&e)[V], float (&xh)[V], float (&a)[V], float (&dh)[V]) {
+      const bool in = V > 1 || c < units;
+      read_unit_or_0<T, V>(in_x, c, in, xh);
+      if constexpr (kMode != kPreNorm) {
+        read_unit_or_0<T, V>(in_y, c, in, yh);
+        if constexpr (kMode == kFullGate) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) a[j] = 0.f;
+          if (in) read_param<T, V>(in_g, p.gate_f32, c, a);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          yh[j] *= ry;
+          a[j] = kMode == kFullGate ? act_of(a[j], p.act) : tok;
+          xh[j] = fmaf(a[j] * pw[i * V + j], yh[j], xh[j]);
+        }
+      }
+      if (p.dxn) read_unit_or_0<T, V>(in_dx, c, in, e);
+      else
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = 0.f;
+      if (p.dh) {
+        read_unit_or_0<T, V>(in_dh, c, in, dh);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          xh[j] *= rx;
+          e[j] = fmaf(rx * dh[j], vo[i * V + j], e[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) xh[j] = dh[j] = 0.f;
+      }
+    };
+    float sums[3] = {0.f, 0.f, 0.f};  // C, A, B / r(x'); A and B without the row's own gate
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (V > 1 && c >= units) continue;
+      float yh[V], e[V], xh[V], a[V], dh[V];
+      read(i, c, yh, e, xh, a, dh);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        sums[0] = fmaf(dh[j] * vo[i * V + j], xh[j], sums[0]);
+        if constexpr (kMode != kPreNorm) {
+          const float q = pw[i * V + j] * yh[j] * (kMode == kFullGate ? a[j] : 1.f);
+          sums[1] = fmaf(q, e[j], sums[1]);
+          sums[2] = fmaf(q, xh[j], sums[2]);
+        }
+      }
+    }
+    block_sum(sums, scratch[odd]);
+    // Every thread is past the previous row's last read of its slot.
+    if (threadIdx.x == 0 && slots > 1 && !ring.dead && row >= gridDim.x) {
+      const long long next = row + static_cast<long long>(slots - 1) * gridDim.x;
+      if (next < p.rows) ring.fetch(slot == 0 ? slots - 1 : slot - 1, next);
+    }
+    const float c1 = rx * (sums[0] * inv_d);  // dx = e - c1 xh
+    const float qdx = sums[1] - c1 * sums[2];
+    const float m = qdx * inv_d * tok;        // mean(t yh)
+    if (kMode == kSharedGate && p.gate_mode == kGateToken && threadIdx.x == 0) {
+      const float d = qdx * act_slope(tok, p.act);
+      if (p.gate_f32) static_cast<float*>(p.dgate_row)[row] = d;
+      else static_cast<T*>(p.dgate_row)[row] = from_float<T>(d);
+    }
+    T* dx_out = static_cast<T*>(p.dx) + row * D;
+    T* dy_out = static_cast<T*>(p.dy) + row * D;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (V > 1 && c >= units) continue;
+      const bool in = V > 1 || c < units;
+      float yh[V], e[V], xh[V], a[V], dh[V];
+      read(i, c, yh, e, xh, a, dh);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        e[j] = fmaf(-c1, xh[j], e[j]);  // dx
+        dv[i * V + j] = fmaf(dh[j], xh[j], dv[i * V + j]);
+      }
+      if (in) write_unit<T, V>(dx_out, c, e);
+      if constexpr (kMode != kPreNorm) {
+        float dg[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float ad = a[j] * e[j];
+          acc[i * V + j] = fmaf(ad, yh[j], acc[i * V + j]);
+          if constexpr (kMode == kFullGate) dg[j] = pw[i * V + j] * yh[j] * e[j] * act_slope(a[j], p.act);
+          yh[j] = ry * fmaf(ad, pw[i * V + j], -yh[j] * m);  // dy
+        }
+        if (in) write_unit<T, V>(dy_out, c, yh);
+        if constexpr (kMode == kFullGate) {
+          if (!in) continue;
+          if (p.gate_f32 && sizeof(T) == 2) {
+            float* out = static_cast<float*>(p.dgate_row) + row * D;
+            if constexpr (V == 1) {
+              out[c] = dg[0];
+            } else {
+#pragma unroll
+              for (int q = 0; q < V / 4; ++q) write_unit<float, 4>(out, c * (V / 4) + q, dg + 4 * q);
+            }
+          } else {
+            write_unit<T, V>(static_cast<T*>(p.dgate_row) + row * D, c, dg);
+          }
+        }
+      }
+    }
+    if (slots == 1) {
+      __syncthreads();
+      const long long next = row + gridDim.x;
+      if (threadIdx.x == 0 && !ring.dead && next < p.rows) ring.fetch(0, next);
+    } else if (blockDim.x == 32) {
+      __syncwarp();
+    }
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+    odd ^= 1;
+  }
+  float* part = p.partial + static_cast<long long>(blockIdx.x) * D;
+  const long long slice = static_cast<long long>(gridDim.x) * D;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c >= units) continue;
+    if constexpr (V == 1) {
+      if (kMode != kPreNorm) part[c] = acc[i];
+      if (p.dh) part[slice + c] = dv[i];
+    } else {
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        if (kMode != kPreNorm) write_unit<float, 4>(part, c * (V / 4) + q, acc + i * V + 4 * q);
+        if (p.dh) write_unit<float, 4>(part + slice, c * (V / 4) + q, dv + i * V + 4 * q);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ wide rows
+template <typename T>
+__device__ __forceinline__ float param1(const void* p, int f32, long long at) {
+  return f32 ? __ldg(static_cast<const float*>(p) + at) : as_float(static_cast<const T*>(p)[at]);
+}
+
+template <typename T>
+__device__ __forceinline__ float gate1(const NormParams& p, long long row, int col, float tok) {
+  if (p.gate_mode != kGateChannel && p.gate_mode != kGateFull) return tok;
+  return act_of(param1<T>(p.gate, p.gate_f32, p.gate_mode == kGateFull ? row * p.dim + col : col), p.act);
+}
+
+// Backward of rows wider than the ring's registers hold (dim > 8192): a thread
+// owns elements threadIdx.x + i * blockDim.x, read from global memory.
+template <typename T, int kE>
 __global__ void __launch_bounds__(kMaxThreads) norm_bwd_kernel(const NormParams p) {
-  __shared__ float scratch[4 * 32];
+  __shared__ float scratch[3 * 32];
   const int D = p.dim;
   const float inv_d = 1.f / static_cast<float>(D);
-  float dw[kChunks][8], dv[kChunks][8], dg[kChunks][8];
+  float acc[kE], dv[kE];
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = dv[i][j] = dg[i][j] = 0.f;
-
+  for (int i = 0; i < kE; ++i) acc[i] = dv[i] = 0.f;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const long long at = row * D;
-    Raw8<T> rx_[kChunks], ry_[kChunks], rdx[kChunks], rdh[kChunks];
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      rx_[i] = load8<T, kVec>(static_cast<const T*>(p.x) + at, col, D);
-      if (p.y) ry_[i] = load8<T, kVec>(static_cast<const T*>(p.y) + at, col, D);
-      if (p.dxn) rdx[i] = load8<T, kVec>(static_cast<const T*>(p.dxn) + at, col, D);
-      if (p.dh) rdh[i] = load8<T, kVec>(static_cast<const T*>(p.dh) + at, col, D);
-    }
     const float ry = p.y ? p.rstd_y[row] : 0.f;
     const float rx = p.dh ? p.rstd_x[row] : 0.f;
     const float tok = token_gate<T>(p, row);
-    // Q = s n (the gate left out when it is the row's own), e = dx' + r(x') u, xh
-    auto chunk = [&](int i, float (&yh)[8], float (&w)[8], float (&a)[8], float (&e)[8], float (&xh)[8],
-                     float (&dhv)[8], float (&v)[8]) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      float xs[8];
-      unpack(rx_[i], xs);
+    float yh[kE], e[kE], xh[kE];
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const int col = threadIdx.x + i * blockDim.x;
+      const bool in_row = col < D;
+      xh[i] = in_row ? as_float(static_cast<const T*>(p.x)[at + col]) : 0.f;
+      yh[i] = in_row && p.y ? as_float(static_cast<const T*>(p.y)[at + col]) * ry : 0.f;
+      e[i] = in_row && p.dxn ? as_float(static_cast<const T*>(p.dxn)[at + col]) : 0.f;
+    }
+    float sums[3] = {0.f, 0.f, 0.f};  // C, A, B / r(x'); A and B without the row's own gate
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const int col = threadIdx.x + i * blockDim.x;
+      if (col >= D) continue;
+      float q = 0.f;
       if (p.y) {
-        unpack(ry_[i], yh);
-        load_param<T, kVec>(p.w, p.w_f32, 0, col, D, w);
-        load_gate<T, kVec>(p, row, col, tok, a);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          yh[j] *= ry;
-          w[j] = (w[j] + p.offset) * p.scale;
-          xs[j] = fmaf(a[j], w[j] * yh[j], xs[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) yh[j] = w[j] = a[j] = 0.f;
+        const float a = gate1<T>(p, row, col, tok);
+        q = (param1<T>(p.w, p.w_f32, col) + p.offset) * p.scale * yh[i];
+        xh[i] = fmaf(a, q, xh[i]);
+        if (p.gate_mode != kGateToken) q *= a;
       }
-      if (p.dxn) unpack(rdx[i], e);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = 0.f;
       if (p.dh) {
-        unpack(rdh[i], dhv);
-        load_param<T, kVec>(p.v, p.w_f32, 0, col, D, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          xh[j] = xs[j] * rx;
-          e[j] = fmaf(rx * dhv[j], v[j] + p.offset, e[j]);
-        }
+        const float u = as_float(static_cast<const T*>(p.dh)[at + col]) * (param1<T>(p.v, p.w_f32, col) + p.offset);
+        xh[i] *= rx;
+        e[i] = fmaf(rx, u, e[i]);
+        sums[0] = fmaf(u, xh[i], sums[0]);
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xh[j] = dhv[j] = v[j] = 0.f;
+        xh[i] = 0.f;
       }
-    };
-    const bool own_gate = p.gate_mode == kGateToken;  // act(g) is one number of the row
-    float sums[3] = {0.f, 0.f, 0.f};                  // C, A, B
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      float yh[8], w[8], a[8], e[8], xh[8], dhv[8], v[8];
-      chunk(i, yh, w, a, e, xh, dhv, v);
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = w[j] * yh[j] * (own_gate ? 1.f : a[j]);
-        if (col + j < D) {
-          sums[0] = fmaf(dhv[j] * (v[j] + p.offset), xh[j], sums[0]);
-          sums[1] = fmaf(q, e[j], sums[1]);
-          sums[2] = fmaf(q, rx * xh[j], sums[2]);
-        }
-      }
+      sums[1] = fmaf(q, e[i], sums[1]);
+      sums[2] = fmaf(q, xh[i], sums[2]);
     }
     block_sum(sums, scratch);
-    const float c = sums[0] * inv_d;
-    const float qdx = sums[1] - c * sums[2];  // sum of Q dx
-    const float m = qdx * inv_d * (own_gate ? tok : 1.f);  // mean(t yh)
-    if (own_gate && threadIdx.x == 0) {
+    const float c1 = rx * (sums[0] * inv_d);
+    const float qdx = sums[1] - c1 * sums[2];
+    const float m = qdx * inv_d * tok;
+    if (p.gate_mode == kGateToken && threadIdx.x == 0) {
       const float d = qdx * act_slope(tok, p.act);
       if (p.gate_f32) static_cast<float*>(p.dgate_row)[row] = d;
       else static_cast<T*>(p.dgate_row)[row] = from_float<T>(d);
     }
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int col = (threadIdx.x + i * blockDim.x) * 8;
-      float yh[8], w[8], a[8], e[8], xh[8], dhv[8], v[8];
-      chunk(i, yh, w, a, e, xh, dhv, v);
-      float dx[8], dy[8], dgr[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dx[j] = fmaf(-rx * c, xh[j], e[j]);
-        const float t = a[j] * dx[j];  // without s (w + o)
-        dy[j] = ry * (t * w[j] - yh[j] * m);
-        dw[i][j] = fmaf(p.scale * t, yh[j], dw[i][j]);
-        dv[i][j] = fmaf(dhv[j], xh[j], dv[i][j]);
-        dgr[j] = w[j] * yh[j] * dx[j] * act_slope(a[j], p.act);
-        dg[i][j] += dgr[j];
-      }
-      if (p.dx) store8<T, kVec>(static_cast<T*>(p.dx) + at, col, D, dx);
-      if (p.y) store8<T, kVec>(static_cast<T*>(p.dy) + at, col, D, dy);
-      if (p.gate_mode == kGateFull) {
-        if (p.gate_f32) store8<float, kVec>(static_cast<float*>(p.dgate_row) + at, col, D, dgr);
-        else store8<T, kVec>(static_cast<T*>(p.dgate_row) + at, col, D, dgr);
+    for (int i = 0; i < kE; ++i) {
+      const int col = threadIdx.x + i * blockDim.x;
+      if (col >= D) continue;
+      const float dx = fmaf(-c1, xh[i], e[i]);
+      if (p.dh) dv[i] = fmaf(as_float(static_cast<const T*>(p.dh)[at + col]), xh[i], dv[i]);
+      static_cast<T*>(p.dx)[at + col] = from_float<T>(dx);
+      if (p.y) {
+        const float a = gate1<T>(p, row, col, tok);
+        const float w = (param1<T>(p.w, p.w_f32, col) + p.offset) * p.scale;
+        // a channel gate's act is a factor of the whole sum (norm_reduce_kernel)
+        acc[i] = fmaf(p.gate_mode == kGateChannel ? dx : a * dx, yh[i], acc[i]);
+        static_cast<T*>(p.dy)[at + col] = from_float<T>(ry * fmaf(a * dx, w, -yh[i] * m));
+        if (p.gate_mode == kGateFull) {
+          const float d = w * yh[i] * dx * act_slope(a, p.act);
+          if (p.gate_f32) static_cast<float*>(p.dgate_row)[at + col] = d;
+          else static_cast<T*>(p.dgate_row)[at + col] = from_float<T>(d);
+        }
       }
     }
     __syncthreads();  // scratch is reused by the next row
@@ -306,69 +731,181 @@ __global__ void __launch_bounds__(kMaxThreads) norm_bwd_kernel(const NormParams 
   const long long slice = static_cast<long long>(gridDim.x) * D;
   float* part = p.partial + static_cast<long long>(blockIdx.x) * D;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const int col = (threadIdx.x + i * blockDim.x) * 8;
-    if (p.y) store8<float, kVec>(part, col, D, dw[i]);
-    if (p.dh) store8<float, kVec>(part + slice, col, D, dv[i]);
-    if (p.gate_mode == kGateChannel) store8<float, kVec>(part + 2 * slice, col, D, dg[i]);
+  for (int i = 0; i < kE; ++i) {
+    const int col = threadIdx.x + i * blockDim.x;
+    if (col >= D) continue;
+    if (p.y) part[col] = acc[i];
+    if (p.dh) part[slice + col] = dv[i];
   }
 }
 
+// Column sums of the blocks' partial sums, and the gradients they stand for:
+// with S = sum act(g) dx yh (act(g) left out for a channel gate),
+//   dw = s S  (s act(g) S for a channel gate),  dgate = s (w + o) act'(g) S.
+// 32 columns a block, 32 warps over the partials, in order (8 warps a block
+// took 11 us for 296 partials of 4096 columns: a chain of 37 reads each).
 struct ReduceParams {
-  const float* partial;  // [3][blocks][D]
-  void* out[3];          // null: not wanted
-  int f32[3];
+  const float* partial;
+  const void *w, *gate;
+  void *dw, *dv, *dgate;  // null: not wanted
+  int w_f32, gate_f32, act;
+  float scale, offset;
   int blocks, dim;
 };
 
-// Column sums of the blocks' partial sums: 32 columns a block, 8 warps over
-// the partials, in order.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const ReduceParams p) {
-  __shared__ float sums[8][33];
-  const int which = blockIdx.y;
-  if (!p.out[which]) return;
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const ReduceParams p) {
+  __shared__ float sums[32][33];
+  const bool second = blockIdx.y == 1;
+  if (second ? !p.dv : !p.dw) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
-  const float* src = p.partial + static_cast<long long>(which) * p.blocks * p.dim;
+  const float* src = p.partial + (second ? static_cast<long long>(p.blocks) * p.dim : 0) + col;
   float s = 0.f;
   if (col < p.dim)
-    for (int b = warp; b < p.blocks; b += 8) s += src[static_cast<long long>(b) * p.dim + col];
+#pragma unroll 8
+    for (int b = warp; b < p.blocks; b += 32) s += src[static_cast<long long>(b) * p.dim];
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < p.dim) {
-    s = 0.f;
+  if (warp != 0 || col >= p.dim) return;
+  s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += sums[w][lane];
-    if (p.f32[which]) static_cast<float*>(p.out[which])[col] = s;
-    else static_cast<T*>(p.out[which])[col] = from_float<T>(s);
+  for (int w = 0; w < 32; ++w) s += sums[w][lane];
+  auto store = [&](void* out, int f32, float v) {
+    if (f32) static_cast<float*>(out)[col] = v;
+    else static_cast<T*>(out)[col] = from_float<T>(v);
+  };
+  if (second) {
+    store(p.dv, p.w_f32, s);
+    return;
+  }
+  s *= p.scale;
+  if (p.dgate) {
+    const float a = act_of(param1<T>(p.gate, p.gate_f32, col), p.act);
+    store(p.dgate, p.gate_f32, s * (param1<T>(p.w, p.w_f32, col) + p.offset) * act_slope(a, p.act));
+    s *= a;
+  }
+  store(p.dw, p.w_f32, s);
+}
+
+// ------------------------------------------------------------------ launches
+int threads_for(int items) { return std::max(32, (items + 31) / 32 * 32); }
+
+constexpr int kRingBytes = 224 * 1024;  // shared memory of an SM the rings may take, over its resident blocks
+constexpr int kMaxSlots = 8;
+
+// Blocks of a ring kernel on one SM, and how many row slots each has.
+struct RingShape {
+  int threads, resident, slots, smem;
+};
+RingShape ring_shape(int dim, int per_thread, int max_threads_sm, size_t slot_bytes) {
+  RingShape r;
+  r.threads = threads_for((dim + per_thread - 1) / per_thread);
+  r.resident = std::max(1, std::min(16, max_threads_sm / r.threads));
+  const size_t share = kRingBytes / r.resident - 1024 - 1024;  // static scratch and the system's own part
+  r.slots = static_cast<int>(std::min<size_t>(kMaxSlots, share / (slot_bytes + 8)));
+  r.smem = r.slots * static_cast<int>(slot_bytes + 8);
+  return r;
+}
+
+// Opts a kernel into its dynamic shared memory, once a device.
+template <typename K>
+cudaError_t allow_smem(K kernel, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes - 2048);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
+
+template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
+cudaError_t launch_fwd_ring(const NormParams& p, const RingShape& r, int sms, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{0};
+  auto kernel = norm_fwd_ring_kernel<T, V, kE, kMode, kThreads, kBlocks>;
+  const cudaError_t e = allow_smem(kernel, done);
+  if (e != cudaSuccess) return e;
+  const int grid = static_cast<int>(std::min<long long>(p.rows, static_cast<long long>(sms) * r.resident));
+  kernel<<<grid, r.threads, r.smem, s>>>(p, r.slots);
+  return cudaSuccess;
+}
+
+template <typename T, int V, int kMode, int kThreads, int kBlocks>
+cudaError_t launch_bwd_ring(const NormParams& p, const RingShape& r, int blocks, cudaStream_t s) {
+  static std::atomic<unsigned long long> done{0};
+  auto kernel = norm_bwd_ring_kernel<T, V, 16, kMode, kThreads, kBlocks>;
+  const cudaError_t e = allow_smem(kernel, done);
+  if (e != cudaSuccess) return e;
+  kernel<<<blocks, r.threads, r.smem, s>>>(p, r.slots);
+  return cudaSuccess;
+}
+
+int mode_of(const NormParams& p) {
+  return !p.y ? kPreNorm : (p.gate_mode == GMM_GATE_MODE_FULL ? kFullGate : kSharedGate);
+}
+
+// Bytes of a slot that holds `inputs` rows of the data type and, with a gate
+// per element, one of the gate's.
+size_t slot_bytes(const NormParams& p, int es, bool vec, int inputs) {
+  const uint32_t gate = p.gate_mode == GMM_GATE_MODE_FULL ? p.dim * (p.gate_f32 ? 4 : es) : 0;
+  return static_cast<size_t>(row_pitch(p.dim * es, vec)) * inputs + (gate ? row_pitch(gate, vec) : 0);
+}
+
+template <typename T, int V, int kE, int kThreads, int kBlocks>
+cudaError_t fwd_ring_mode(const NormParams& p, int sms, cudaStream_t s) {
+  const RingShape r = ring_shape(p.dim, kE, kThreads * kBlocks, slot_bytes(p, sizeof(T), V > 1, p.y ? 2 : 1));
+  switch (mode_of(p)) {
+    case kPreNorm: return launch_fwd_ring<T, V, kE, kPreNorm, kThreads, kBlocks>(p, r, sms, s);
+    case kSharedGate: return launch_fwd_ring<T, V, kE, kSharedGate, kThreads, kBlocks>(p, r, sms, s);
+    default: return launch_fwd_ring<T, V, kE, kFullGate, kThreads, kBlocks>(p, r, sms, s);
   }
 }
 
-int chunks_of(int dim) { return (dim + 7) / 8; }
-int threads_of(int dim, int per) { return std::max(32, (chunks_of(dim) + 32 * per - 1) / (32 * per) * 32); }
+template <typename T, int V>
+cudaError_t fwd_ring_width(const NormParams& p, int sms, cudaStream_t s) {
+  if (p.dim <= 4096) return fwd_ring_mode<T, V, 8, 512, 2>(p, sms, s);
+  if (p.dim <= 8192) return fwd_ring_mode<T, V, 8, 1024, 1>(p, sms, s);
+  return fwd_ring_mode<T, V, 16, 1024, 1>(p, sms, s);
+}
+
+template <typename T>
+cudaError_t launch_fwd(const NormParams& p, bool vec, int sms, cudaStream_t s) {
+  return vec ? fwd_ring_width<T, kV<T>>(p, sms, s) : fwd_ring_width<T, 1>(p, sms, s);
+}
+
+// The ring's backward kernels keep 16 elements a thread (their parameters and
+// sums over rows in registers) in at most 512 threads.
+constexpr int kMaxRingBwdDim = 8192;
 
 // Blocks of the backward pass: what is resident at once, so that every block
 // adds up as many rows as possible before it leaves its partial sums.
 int bwd_blocks(int64_t rows, int dim, int sms) {
-  const int per = dim <= 8 * kMaxThreads ? 1 : (dim <= 16 * kMaxThreads ? 2 : 4);
-  const int resident = std::max(1, std::min(16, 512 / threads_of(dim, per)));
+  const int threads = threads_for((dim + 15) / 16);  // one block an SM past kMaxRingBwdDim
+  const int resident = std::max(1, std::min(16, 512 / threads));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sms) * resident)));
 }
 
-template <typename T, bool kVec>
-void launch_fwd(const NormParams& p, int sms, cudaStream_t s) {
-  const int grid = static_cast<int>(std::min<long long>(p.rows, 64LL * sms));
-  if (p.dim <= 8 * kMaxThreads) norm_fwd_kernel<T, 1, kVec><<<grid, threads_of(p.dim, 1), 0, s>>>(p);
-  else if (p.dim <= 16 * kMaxThreads) norm_fwd_kernel<T, 2, kVec><<<grid, threads_of(p.dim, 2), 0, s>>>(p);
-  else norm_fwd_kernel<T, 4, kVec><<<grid, threads_of(p.dim, 4), 0, s>>>(p);
+template <typename T, int V, int kThreads, int kBlocks>
+cudaError_t bwd_ring_mode(const NormParams& p, int blocks, cudaStream_t s) {
+  const int inputs = 1 + (p.y ? 1 : 0) + (p.dxn ? 1 : 0) + (p.dh ? 1 : 0);
+  const RingShape r = ring_shape(p.dim, 16, kThreads * kBlocks, slot_bytes(p, sizeof(T), V > 1, inputs));
+  switch (mode_of(p)) {
+    case kPreNorm: return launch_bwd_ring<T, V, kPreNorm, kThreads, kBlocks>(p, r, blocks, s);
+    case kSharedGate: return launch_bwd_ring<T, V, kSharedGate, kThreads, kBlocks>(p, r, blocks, s);
+    default: return launch_bwd_ring<T, V, kFullGate, kThreads, kBlocks>(p, r, blocks, s);
+  }
 }
 
-template <typename T, bool kVec>
-void launch_bwd(const NormParams& p, int blocks, cudaStream_t s) {
-  if (p.dim <= 8 * kMaxThreads) norm_bwd_kernel<T, 1, kVec><<<blocks, threads_of(p.dim, 1), 0, s>>>(p);
-  else if (p.dim <= 16 * kMaxThreads) norm_bwd_kernel<T, 2, kVec><<<blocks, threads_of(p.dim, 2), 0, s>>>(p);
-  else norm_bwd_kernel<T, 4, kVec><<<blocks, threads_of(p.dim, 4), 0, s>>>(p);
+template <typename T>
+cudaError_t launch_bwd(const NormParams& p, bool vec, int blocks, cudaStream_t s) {
+  if (p.dim > kMaxRingBwdDim) {
+    norm_bwd_kernel<T, kMaxNormDim / kMaxThreads><<<blocks, kMaxThreads, 0, s>>>(p);
+    return cudaSuccess;
+  }
+  if (p.dim <= 4096) return vec ? bwd_ring_mode<T, kV<T>, 256, 2>(p, blocks, s) : bwd_ring_mode<T, 1, 256, 2>(p, blocks, s);
+  return vec ? bwd_ring_mode<T, kV<T>, 512, 1>(p, blocks, s) : bwd_ring_mode<T, 1, 512, 1>(p, blocks, s);
 }
 
 bool on(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -390,6 +927,14 @@ int check_common(int64_t rows, int64_t dim, int dtype, int weight_dtype, int gat
 }
 
 }  // namespace
+
+int norm_device_error(int* status, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_norm_error, sizeof(int));
+  const int zero = 0;
+  if (e == cudaSuccess && clear && *status) e = cudaMemcpyToSymbol(g_norm_error, &zero, sizeof(int));
+  return e == cudaSuccess ? GMM_OK : set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
+}
+
 }  // namespace gmm_sm100
 
 extern "C" {
@@ -418,17 +963,13 @@ int gmm_sm100_post_norm(const void* y, const void* x, const void* weight, const 
   p.w_f32 = weight_dtype == GMM_DTYPE_F32; p.gate_f32 = gate_dtype == GMM_DTYPE_F32;
   p.gate_mode = gate_mode; p.act = gate_act;
   p.scale = residual_scale; p.eps = eps; p.offset = weight_offset;
-  const bool vec = dim % 8 == 0 && on(y, 16) && on(x, 16) && on(x_new, 16) && on(h, 16) && on(weight, 16) &&
-                   on(next_weight, 16) && (gate_mode == GMM_GATE_MODE_TOKEN || on(gate, 16));
+  const bool vec = dim % (16 / static_cast<int64_t>(es)) == 0 && on(y, 16) && on(x, 16) && on(x_new, 16) && on(h, 16) &&
+                   on(weight, 16) && on(next_weight, 16) && (gate_mode == GMM_GATE_MODE_TOKEN || on(gate, 16));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto t) {
-    using T = decltype(t);
-    vec ? launch_fwd<T, true>(p, sms, s) : launch_fwd<T, false>(p, sms, s);
-  };
-  if (dtype == GMM_DTYPE_F32) go(float{});
-  else if (dtype == GMM_DTYPE_BF16) go(__nv_bfloat16{});
-  else go(__half{});
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = dtype == GMM_DTYPE_F32    ? launch_fwd<float>(p, vec, sms, s)
+                  : dtype == GMM_DTYPE_BF16 ? launch_fwd<__nv_bfloat16>(p, vec, sms, s)
+                                            : launch_fwd<__half>(p, vec, sms, s);
+  if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? GMM_OK : set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -437,7 +978,7 @@ size_t gmm_sm100_post_norm_backward_workspace_size(int64_t rows, int64_t dim) {
   if (rows <= 0 || dim <= 0 || dim > kMaxNormDim) return 0;
   int sms = 0;
   if (current_sm_count(&sms)) return 0;
-  return 3 * sizeof(float) * static_cast<size_t>(bwd_blocks(rows, static_cast<int>(dim), sms)) * dim;
+  return 2 * sizeof(float) * static_cast<size_t>(bwd_blocks(rows, static_cast<int>(dim), sms)) * dim;
 }
 
 int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weight, const void* gate,
@@ -469,8 +1010,7 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
     return set_error(GMM_ERR_ALIGNMENT, "a pointer is not aligned to its element size");
   int sms = 0;
   if (int rc = current_sm_count(&sms)) return rc;
-  const int blocks = bwd_blocks(rows, static_cast<int>(dim), sms);
-  const size_t need = 3 * sizeof(float) * static_cast<size_t>(blocks) * dim;
+  const size_t need = gmm_sm100_post_norm_backward_workspace_size(rows, dim);
   if (!workspace || workspace_bytes < need || !on(workspace, 16)) {
     char msg[96];
     std::snprintf(msg, sizeof msg, "workspace needs %zu bytes (16-byte aligned), got %zu", need, workspace_bytes);
@@ -485,28 +1025,35 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
   p.w_f32 = weight_dtype == GMM_DTYPE_F32; p.gate_f32 = gate_dtype == GMM_DTYPE_F32;
   p.gate_mode = gate_mode; p.act = gate_act;
   p.scale = residual_scale; p.offset = weight_offset;
-  const bool vec = dim % 8 == 0 && on(y, 16) && on(x, 16) && on(dx_new, 16) && on(dh, 16) && on(dy, 16) && on(dx, 16) &&
-                   on(weight, 16) && on(next_weight, 16) &&
+  const bool vec = dim % (16 / static_cast<int64_t>(es)) == 0 && on(y, 16) && on(x, 16) && on(dx_new, 16) && on(dh, 16) &&
+                   on(dy, 16) && on(dx, 16) && on(weight, 16) && on(next_weight, 16) &&
                    (gate_mode == GMM_GATE_MODE_TOKEN || (on(gate, 16) && on(dgate, 16)));
+  const int blocks = bwd_blocks(rows, p.dim, sms);
   ReduceParams r = {};
   r.partial = p.partial;
-  r.out[0] = y ? dweight : nullptr;
-  r.out[1] = dh ? dnext_weight : nullptr;
-  r.out[2] = gate_mode == GMM_GATE_MODE_CHANNEL ? dgate : nullptr;
-  r.f32[0] = r.f32[1] = p.w_f32;
-  r.f32[2] = p.gate_f32;
+  r.w = weight;
+  r.gate = gate;
+  r.dw = y ? dweight : nullptr;
+  r.dv = dh ? dnext_weight : nullptr;
+  r.dgate = gate_mode == GMM_GATE_MODE_CHANNEL ? dgate : nullptr;
+  r.w_f32 = p.w_f32;
+  r.gate_f32 = p.gate_f32;
+  r.act = gate_act;
+  r.scale = residual_scale;
+  r.offset = weight_offset;
   r.blocks = blocks;
   r.dim = p.dim;
-  const dim3 rgrid((p.dim + 31) / 32, 3);
+  const dim3 rgrid((p.dim + 31) / 32, 2);
   auto go = [&](auto t) {
     using T = decltype(t);
-    vec ? launch_bwd<T, true>(p, blocks, s) : launch_bwd<T, false>(p, blocks, s);
-    norm_reduce_kernel<T><<<rgrid, 256, 0, s>>>(r);
+    const cudaError_t e = launch_bwd<T>(p, vec, blocks, s);
+    if (e != cudaSuccess) return e;
+    norm_reduce_kernel<T><<<rgrid, 1024, 0, s>>>(r);
+    return cudaGetLastError();
   };
-  if (dtype == GMM_DTYPE_F32) go(float{});
-  else if (dtype == GMM_DTYPE_BF16) go(__nv_bfloat16{});
-  else go(__half{});
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = dtype == GMM_DTYPE_F32    ? go(float{})
+                        : dtype == GMM_DTYPE_BF16 ? go(__nv_bfloat16{})
+                                                  : go(__half{});
   return e == cudaSuccess ? GMM_OK : set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
 }
 
