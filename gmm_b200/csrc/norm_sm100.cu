@@ -327,30 +327,35 @@ struct RowRing {
 };
 
 // s (w + o), times act(g) of a channel gate; v + o.  Zero past the row's end.
+// All loads first: they come from DRAM, one latency for all of them.
 template <typename T, int V, int kE, int kMode>
 __device__ __forceinline__ void row_params(const NormParams& p, bool with_v, float (&pw)[kE], float (&vo)[kE]) {
   const int units = p.dim / V;
+  const bool channel = kMode == kSharedGate && p.gate_mode == kGateChannel;
+  float g[kMode == kSharedGate ? kE : 1];
+#pragma unroll
+  for (int j = 0; j < kE; ++j) pw[j] = vo[j] = 0.f;
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
+    if (kMode != kPreNorm && c < units) read_param<T, V>(p.w, p.w_f32, c, pw + i * V);
+    if (with_v && c < units) read_param<T, V>(p.v, p.w_f32, c, vo + i * V);
+    if constexpr (kMode == kSharedGate) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) pw[i * V + j] = vo[i * V + j] = 0.f;
-    if (c >= units) continue;
-    if constexpr (kMode != kPreNorm) {
-      read_param<T, V>(p.w, p.w_f32, c, pw + i * V);
-#pragma unroll
-      for (int j = 0; j < V; ++j) pw[i * V + j] = (pw[i * V + j] + p.offset) * p.scale;
-      if (kMode == kSharedGate && p.gate_mode == kGateChannel) {
-        float g[V];
-        read_param<T, V>(p.gate, p.gate_f32, c, g);
-#pragma unroll
-        for (int j = 0; j < V; ++j) pw[i * V + j] *= act_of(g[j], p.act);
-      }
+      for (int j = 0; j < V; ++j) g[i * V + j] = 0.f;
+      if (channel && c < units) read_param<T, V>(p.gate, p.gate_f32, c, g + i * V);
     }
-    if (with_v) {
-      read_param<T, V>(p.v, p.w_f32, c, vo + i * V);
+  }
 #pragma unroll
-      for (int j = 0; j < V; ++j) vo[i * V + j] += p.offset;
+  for (int i = 0; i < kE / V; ++i) {
+    const bool in = threadIdx.x + i * blockDim.x < units;
+#pragma unroll
+    for (int j = i * V; j < (i + 1) * V; ++j) {
+      if (kMode != kPreNorm) {
+        pw[j] = in ? (pw[j] + p.offset) * p.scale : 0.f;
+        if (kMode == kSharedGate && channel) pw[j] *= act_of(g[j], p.act);
+      }
+      vo[j] = in && with_v ? vo[j] + p.offset : 0.f;
     }
   }
 }
