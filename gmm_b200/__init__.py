@@ -160,13 +160,11 @@ def _register_fakes() -> None:
 
     def _post_norm_fake(y, x, weight, gate, next_weight, gate_act, residual_scale, eps, weight_offset, keep):
         rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-        stat = [torch.empty(rows if keep and t is not None else 0, dtype=torch.float32, device=x.device)
-                for t in (y, next_weight)]
         outs = [torch.empty(x.shape if t is not None else (0,), dtype=x.dtype, device=x.device)
                 for t in (y, next_weight)]
-        return outs[0], outs[1], stat[0], stat[1]
+        return outs[0], outs[1], torch.empty((2, rows) if keep else (0,), dtype=torch.float32, device=x.device)
 
-    def _post_norm_backward_fake(y, x, weight, gate, next_weight, rstd_y, rstd_x, dx_new, dh, gate_act,
+    def _post_norm_backward_fake(y, x, weight, gate, next_weight, stats, dx_new, dh, gate_act,
                                  residual_scale, weight_offset):
         like = (y, x, weight if y is not None else None, gate, next_weight)
         return [torch.empty((0,) if t is None else t.shape, dtype=(x if t is None else t).dtype, device=x.device)

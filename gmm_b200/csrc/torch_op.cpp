@@ -15,6 +15,8 @@
 //     as documented for trans_b; the reference transposed such a B a second
 //     time (hopper_gmm_forward.cu:442-446).
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -119,6 +121,14 @@ at::Tensor gmm_swiglu(at::Tensor A, at::Tensor B, at::Tensor batch_sizes, bool t
   return D;
 }
 
+// An uninitialised tensor on the current device, straight from the caching
+// allocator: at::empty dispatches again, which costs a small call as much as
+// its launch does.
+at::Tensor device_empty(c10::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(),
+                                              c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt));
+}
+
 // ---------------------------------------------------------------- 8-bit grouped product
 int dtype_code(at::ScalarType t, const char* what) {
   switch (t) {
@@ -154,7 +164,7 @@ at::Tensor check_int8(const at::Tensor& A, const at::Tensor& a_scale, const at::
     TORCH_CHECK(out_dtype != at::kFloat, "gmm_int8 with swiglu gives bf16 / fp16");
     TORCH_CHECK(B.size(1) % 2 == 0, "B must hold gate and up projections of equal width");
   }
-  return at::empty({A.size(0), swiglu ? B.size(1) / 2 : B.size(1)}, A.options().dtype(out_dtype));
+  return device_empty({A.size(0), swiglu ? B.size(1) / 2 : B.size(1)}, out_dtype);
 }
 
 at::Tensor gmm_int8(const at::Tensor& A, const at::Tensor& a_scale, const at::Tensor& B, const at::Tensor& b_scale,
@@ -215,8 +225,8 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, const std:
     k = pos.size(1);
   }
   TORCH_CHECK(out_rows >= 0, "out_rows must not be negative");
-  at::Tensor q = at::empty({out_rows, (x.size(1) + 15) / 16 * 16}, x.options().dtype(at::kChar));
-  at::Tensor scale = at::empty({out_rows}, x.options().dtype(at::kFloat));
+  at::Tensor q = device_empty({out_rows, (x.size(1) + 15) / 16 * 16}, at::kChar);
+  at::Tensor scale = device_empty({out_rows}, at::kFloat);
   const int rc = gmm_sm100_quantize_rows(rows.data_ptr(), dtype, x.size(0), x.size(1),
                                          dst_pos ? pos.data_ptr<int>() : nullptr, static_cast<int>(std::min<int64_t>(k, 1 << 20)),
                                          out_rows, q.data_ptr<int8_t>(), scale.data_ptr<float>(),
@@ -284,35 +294,37 @@ NormArgs check_norm(const OptTensor& y, const at::Tensor& x, const OptTensor& we
 void* ptr(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 OptTensor dense(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : t; }
 
-// (x_new, h, rstd_y, rstd_x); what was not asked for is an empty tensor.
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> post_norm(
-    const OptTensor& y_, const at::Tensor& x_, const OptTensor& weight_, const OptTensor& gate_,
-    const OptTensor& next_weight_, int64_t gate_act, double residual_scale, double eps, double weight_offset,
-    bool keep) {
+// (x_new, h, stats): stats keeps r(y) and r(x_new) of every row, [2, rows];
+// what was not asked for is an empty tensor.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> post_norm(const OptTensor& y_, const at::Tensor& x_,
+                                                         const OptTensor& weight_, const OptTensor& gate_,
+                                                         const OptTensor& next_weight_, int64_t gate_act,
+                                                         double residual_scale, double eps, double weight_offset,
+                                                         bool keep) {
   const NormArgs n = check_norm(y_, x_, weight_, gate_, next_weight_);
   const c10::cuda::CUDAGuard guard(x_.device());
   const OptTensor y = dense(y_), weight = dense(weight_), gate = dense(gate_), next_weight = dense(next_weight_);
   const at::Tensor x = x_.contiguous();
-  const auto stat = x.options().dtype(at::kFloat);
-  at::Tensor x_new = y ? at::empty_like(x) : at::empty({0}, x.options());
-  at::Tensor h = next_weight ? at::empty_like(x) : at::empty({0}, x.options());
-  at::Tensor ry = at::empty({keep && y ? n.rows : 0}, stat), rx = at::empty({keep && next_weight ? n.rows : 0}, stat);
+  const at::ScalarType type = x.scalar_type();
+  at::Tensor x_new = y ? device_empty(x.sizes(), type) : device_empty({0}, type);
+  at::Tensor h = next_weight ? device_empty(x.sizes(), type) : device_empty({0}, type);
+  at::Tensor stats = keep ? device_empty({2, n.rows}, at::kFloat) : device_empty({0}, at::kFloat);
+  float* ry = keep ? stats.data_ptr<float>() : nullptr;
   const int rc = gmm_sm100_post_norm(
       ptr(y), x.data_ptr(), ptr(weight), ptr(gate), ptr(next_weight), n.rows, n.dim, n.dtype, n.weight_dtype,
       n.gate_dtype, n.gate_mode, static_cast<int>(gate_act), static_cast<float>(residual_scale),
       static_cast<float>(eps), static_cast<float>(weight_offset), y ? x_new.data_ptr() : nullptr,
-      next_weight ? h.data_ptr() : nullptr, ry.numel() ? ry.data_ptr<float>() : nullptr,
-      rx.numel() ? rx.data_ptr<float>() : nullptr, c10::cuda::getCurrentCUDAStream(x.get_device()).stream());
+      next_weight ? h.data_ptr() : nullptr, ry, ry ? ry + n.rows : nullptr,
+      c10::cuda::getCurrentCUDAStream(x.get_device()).stream());
   TORCH_CHECK(rc == GMM_OK, gmm_sm100_last_error());
-  return {x_new, h, ry, rx};
+  return {x_new, h, stats};
 }
 
 // (dy, dx, dweight, dgate, dnext_weight); empty where there is nothing to differentiate.
 std::vector<at::Tensor> post_norm_backward(const OptTensor& y_, const at::Tensor& x_, const OptTensor& weight_,
                                            const OptTensor& gate_, const OptTensor& next_weight_,
-                                           const at::Tensor& rstd_y, const at::Tensor& rstd_x,
-                                           const OptTensor& dx_new_, const OptTensor& dh_, int64_t gate_act,
-                                           double residual_scale, double weight_offset) {
+                                           const at::Tensor& stats, const OptTensor& dx_new_, const OptTensor& dh_,
+                                           int64_t gate_act, double residual_scale, double weight_offset) {
   const NormArgs n = check_norm(y_, x_, weight_, gate_, next_weight_);
   const c10::cuda::CUDAGuard guard(x_.device());
   TORCH_CHECK(dx_new_ || dh_, "post_norm_backward needs the gradient of x_new or of h");
@@ -322,25 +334,24 @@ std::vector<at::Tensor> post_norm_backward(const OptTensor& y_, const at::Tensor
                       (*g)->scalar_type() == x_.scalar_type(),
                   "the outputs' gradients must have the rows' shape, dtype and device");
   TORCH_CHECK(!dh_ || next_weight_, "a gradient of h needs next_weight");
-  TORCH_CHECK(rstd_y.is_cuda() && rstd_x.is_cuda() && rstd_y.is_contiguous() && rstd_x.is_contiguous() &&
-                  rstd_y.scalar_type() == at::kFloat && rstd_x.scalar_type() == at::kFloat &&
-                  (!y_ || rstd_y.numel() == n.rows) && (!dh_ || rstd_x.numel() == n.rows),
-              "rstd_y and rstd_x must be the forward pass's");
+  TORCH_CHECK(stats.is_cuda() && stats.get_device() == x_.get_device() && stats.is_contiguous() &&
+                  stats.scalar_type() == at::kFloat && stats.numel() == 2 * n.rows,
+              "stats must be the forward pass's");
   const OptTensor y = dense(y_), weight = dense(weight_), gate = dense(gate_), next_weight = dense(next_weight_),
                   dx_new = dense(dx_new_), dh = dense(dh_);
   const at::Tensor x = x_.contiguous();
-  auto none = [&] { return at::empty({0}, x.options()); };
-  at::Tensor dx = at::empty_like(x);
-  at::Tensor dy = y ? at::empty_like(x) : none();
-  at::Tensor dw = y ? at::empty_like(*weight) : none();
-  at::Tensor dg = gate ? at::empty_like(*gate) : none();
+  const at::ScalarType type = x.scalar_type();
+  auto like = [&](const OptTensor& t, bool wanted = true) {
+    return wanted && t ? device_empty(t->sizes(), t->scalar_type()) : device_empty({0}, type);
+  };
+  at::Tensor dx = device_empty(x.sizes(), type), dy = like(y), dw = like(weight, y.has_value()), dg = like(gate);
   // without dh the next norm's weight gets no gradient
-  at::Tensor dv = next_weight ? (dh ? at::empty_like(*next_weight) : at::zeros_like(*next_weight)) : none();
+  at::Tensor dv = next_weight && !dh ? at::zeros_like(*next_weight) : like(next_weight);
   const size_t ws_bytes = gmm_sm100_post_norm_backward_workspace_size(n.rows, n.dim);
-  at::Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+  at::Tensor ws = device_empty({static_cast<int64_t>(ws_bytes)}, at::kByte);
+  const float* ry = stats.data_ptr<float>();
   const int rc = gmm_sm100_post_norm_backward(
-      ptr(y), x.data_ptr(), ptr(weight), ptr(gate), ptr(next_weight), y ? rstd_y.data_ptr<float>() : nullptr,
-      dh ? rstd_x.data_ptr<float>() : nullptr, ptr(dx_new), ptr(dh), n.rows, n.dim, n.dtype, n.weight_dtype,
+      ptr(y), x.data_ptr(), ptr(weight), ptr(gate), ptr(next_weight), ry, ry + n.rows, ptr(dx_new), ptr(dh), n.rows, n.dim, n.dtype, n.weight_dtype,
       n.gate_dtype, n.gate_mode, static_cast<int>(gate_act), static_cast<float>(residual_scale),
       static_cast<float>(weight_offset), y ? dy.data_ptr() : nullptr, dx.data_ptr(), y ? dw.data_ptr() : nullptr,
       gate ? dg.data_ptr() : nullptr, dh ? dv.data_ptr() : nullptr, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
@@ -371,16 +382,16 @@ class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
                                                 const OptTensor& next_weight, int64_t gate_act, double residual_scale,
                                                 double eps, double weight_offset) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [x_new, h, ry, rx] =
+    auto [x_new, h, stats] =
         post_norm_op().call(y, x, weight, gate, next_weight, gate_act, residual_scale, eps, weight_offset, true);
     ctx->save_for_backward({y.value_or(at::Tensor()), x, weight.value_or(at::Tensor()), gate.value_or(at::Tensor()),
-                            next_weight.value_or(at::Tensor()), ry, rx});
+                            next_weight.value_or(at::Tensor()), stats});
     ctx->saved_data["gate_act"] = gate_act;
     ctx->saved_data["residual_scale"] = residual_scale;
     ctx->saved_data["weight_offset"] = weight_offset;
-    ctx->mark_non_differentiable({ry, rx});
+    ctx->mark_non_differentiable({stats});
     ctx->set_materialize_grads(false);
-    return {x_new, h, ry, rx};
+    return {x_new, h, stats};
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -393,7 +404,7 @@ class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
     if (!dx_new && !dh) return out;
     const OptTensor weight = opt(saved[2]), gate = opt(saved[3]);
     const auto g = post_norm_backward_op().call(
-        y, saved[1], weight, gate, next_weight, saved[5], saved[6], dx_new, dh, ctx->saved_data["gate_act"].toInt(),
+        y, saved[1], weight, gate, next_weight, saved[5], dx_new, dh, ctx->saved_data["gate_act"].toInt(),
         ctx->saved_data["residual_scale"].toDouble(), ctx->saved_data["weight_offset"].toDouble());
     out[1] = g[1];
     if (y) {
@@ -406,7 +417,7 @@ class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
   }
 };
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> post_norm_autograd(
+std::tuple<at::Tensor, at::Tensor, at::Tensor> post_norm_autograd(
     const OptTensor& y, const at::Tensor& x, const OptTensor& weight, const OptTensor& gate,
     const OptTensor& next_weight, int64_t gate_act, double residual_scale, double eps, double weight_offset,
     bool keep) {
@@ -417,19 +428,19 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> post_norm_autograd(
     return post_norm_op().call(y, x, weight, gate, next_weight, gate_act, residual_scale, eps, weight_offset, keep);
   }
   auto out = PostNormGrad::apply(y, x, weight, gate, next_weight, gate_act, residual_scale, eps, weight_offset);
-  return {out[0], out[1], out[2], out[3]};
+  return {out[0], out[1], out[2]};
 }
 
 std::vector<at::Tensor> post_norm_backward_autograd(const OptTensor& y, const at::Tensor& x, const OptTensor& weight,
                                                     const OptTensor& gate, const OptTensor& next_weight,
-                                                    const at::Tensor& rstd_y, const at::Tensor& rstd_x,
-                                                    const OptTensor& dx_new, const OptTensor& dh, int64_t gate_act,
-                                                    double residual_scale, double weight_offset) {
+                                                    const at::Tensor& stats, const OptTensor& dx_new,
+                                                    const OptTensor& dh, int64_t gate_act, double residual_scale,
+                                                    double weight_offset) {
   // reached with gradients on only under create_graph
   TORCH_CHECK(!at::GradMode::is_enabled(), "post_norm has no second derivative (create_graph=True)");
   at::AutoDispatchBelowADInplaceOrView below;
-  return post_norm_backward_op().call(y, x, weight, gate, next_weight, rstd_y, rstd_x, dx_new, dh, gate_act,
-                                      residual_scale, weight_offset);
+  return post_norm_backward_op().call(y, x, weight, gate, next_weight, stats, dx_new, dh, gate_act, residual_scale,
+                                      weight_offset);
 }
 
 }  // namespace gmm_b200
@@ -443,9 +454,9 @@ TORCH_LIBRARY(hopper_gmm_fwd, m) {
         "ScalarType out_dtype, bool swiglu) -> Tensor");
   m.def("quantize_rows(Tensor x, Tensor? dst_pos, int out_rows) -> (Tensor, Tensor)");
   m.def("post_norm(Tensor? y, Tensor x, Tensor? weight, Tensor? gate, Tensor? next_weight, int gate_act, "
-        "float residual_scale, float eps, float weight_offset, bool keep) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("post_norm_backward(Tensor? y, Tensor x, Tensor? weight, Tensor? gate, Tensor? next_weight, Tensor rstd_y, "
-        "Tensor rstd_x, Tensor? dx_new, Tensor? dh, int gate_act, float residual_scale, float weight_offset) "
+        "float residual_scale, float eps, float weight_offset, bool keep) -> (Tensor, Tensor, Tensor)");
+  m.def("post_norm_backward(Tensor? y, Tensor x, Tensor? weight, Tensor? gate, Tensor? next_weight, Tensor stats, "
+        "Tensor? dx_new, Tensor? dh, int gate_act, float residual_scale, float weight_offset) "
         "-> Tensor[]");
 }
 

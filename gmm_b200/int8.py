@@ -48,7 +48,7 @@ def quantize_rows(x: torch.Tensor, dst_pos: Optional[torch.Tensor] = None,
     """
     if out_rows is None:
         out_rows = x.shape[0] * (1 if dst_pos is None else dst_pos.shape[1])
-    return _ops().quantize_rows(x, dst_pos, out_rows)
+    return _ops().quantize_rows.default(x, dst_pos, out_rows)
 
 
 def quantize_experts(w: torch.Tensor, trans_b: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -85,7 +85,7 @@ def gmm_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
            ``silu(gate) * up`` of the scaled sums, ``[num_tokens, dim_out // 2]``
            (bf16 / fp16, ``dim_out`` a multiple of 16).
     """
-    return _ops().gmm_int8(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
+    return _ops().gmm_int8.default(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
 
 
 def gmm_int8_dev(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -95,4 +95,4 @@ def gmm_int8_dev(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
 
     ``a`` has capacity rows; the first ``sum(batch_sizes)`` are used and only
     those rows of the result are written."""
-    return _ops().gmm_int8_dev(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
+    return _ops().gmm_int8_dev.default(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)

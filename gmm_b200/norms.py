@@ -24,16 +24,16 @@ import gmm_b200
 _GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
 
 
-def _ops():
+def _op():
     if not gmm_b200._HAS_C:
         raise RuntimeError("gmm_b200._C is not available. Build with `python -m gmm_b200.build`.")
-    return torch.ops.hopper_gmm_fwd
+    return torch.ops.hopper_gmm_fwd.post_norm.default
 
 
 def pre_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
              weight_offset: float = 0.0) -> torch.Tensor:
     """RMS norm of ``x [..., dim]`` (CUDA, fp32/bf16/fp16, ``dim <= 16384``); ``weight [dim]`` of ``x``'s dtype or fp32."""
-    return _ops().post_norm(None, x, None, None, weight, 0, 1.0, eps, weight_offset, False)[1]
+    return _op()(None, x, None, None, weight, 0, 1.0, eps, weight_offset, False)[1]
 
 
 def post_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
@@ -56,6 +56,6 @@ def post_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     """
     if gate_act not in _GATE_ACTS:
         raise ValueError(f"gate_act must be one of {sorted(_GATE_ACTS)}, got {gate_act!r}")
-    new, h, _, _ = _ops().post_norm(y, residual, weight, gate, next_weight, _GATE_ACTS[gate_act], residual_scale,
-                                    eps, weight_offset, False)
+    new, h, _ = _op()(y, residual, weight, gate, next_weight, _GATE_ACTS[gate_act], residual_scale, eps,
+                        weight_offset, False)
     return new if next_weight is None else (new, h)

@@ -130,9 +130,9 @@ def test_fake_impls():
         leaves = [t.requires_grad_() for t in (x, w, torch.empty(10, 1, dtype=torch.bfloat16, device="cuda"))]
         outs = post_norm(leaves[0], leaves[0], leaves[1], gate=leaves[2], next_weight=leaves[1])
         assert all(o.requires_grad for o in outs)
-        r = torch.empty(10, dtype=torch.float32, device="cuda")
+        stats = torch.empty(2, 10, dtype=torch.float32, device="cuda")
         with torch.no_grad():
-            g = torch.ops.hopper_gmm_fwd.post_norm_backward(x, x, w, leaves[2], None, r, r[:0], outs[0], None, 0, 1.0, 0.0)
+            g = torch.ops.hopper_gmm_fwd.post_norm_backward(x, x, w, leaves[2], None, stats, outs[0], None, 0, 1.0, 0.0)
         assert [tuple(t.shape) for t in g] == [(10, 40), (10, 40), (40,), (10, 1), (0,)]
 
 
