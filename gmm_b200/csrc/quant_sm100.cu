@@ -26,6 +26,53 @@ namespace {
 
 constexpr int kMaxDim = 65536;
 
+// Largest |x| of eight elements, as its fp32 bits: ordered like the values,
+// with NaN above infinity.  16-bit types compare two at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t m = __vmaxu2(__vmaxu2(r.q[0].x & 0x7fff7fffu, r.q[0].y & 0x7fff7fffu),
+                                __vmaxu2(r.q[0].z & 0x7fff7fffu, r.q[0].w & 0x7fff7fffu));
+    const float2 f = unpack2(m, static_cast<const T*>(nullptr));
+    return max(__float_as_uint(f.x), __float_as_uint(f.y));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      m = max(max(max(m, r.q[i].x & 0x7fffffffu), r.q[i].y & 0x7fffffffu),
+              max(r.q[i].z & 0x7fffffffu, r.q[i].w & 0x7fffffffu));
+    return m;
+  }
+}
+
+// rint(x / scale) of eight elements, two's complement bytes.
+//
+// x * inv, inv = 1 / scale rounded, lies within 2^-24 of x / scale (relative,
+// and one more 2^-24 for the division that defines the code), so both round
+// to the same integer unless the product comes within 3 * 2^-24 * 127.5 <
+// 2^-15 of a half.  Adding 1.5 * 2^23 rounds the exact product to an integer
+// and leaves it in the low bits; only chunks with a product that near to a
+// half (1 in 2000) divide.  A division per element made the kernel issue-bound
+// (77 us for 16384 x 4096 bf16 into two places).
+// `divide`: 1 / scale may not be finite.
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale, float inv, bool divide) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t u[8];
+  float half = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float r = fmaf(f[j], inv, kMagic);
+    u[j] = __float_as_uint(r);
+    half = fmaxf(half, fabsf(fmaf(f[j], inv, kMagic - r)));
+  }
+  if (divide || half > 0.5f - 0x1p-15f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = max(-127, min(127, __float2int_rn(__fdiv_rn(f[j], scale))));
+  }
+  return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+}
+
 // One block per row; thread t holds the 8-element chunks t, t + blockDim.x, ...
 template <typename T, int kChunks, bool kVec>
 __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, int dim, int dim_padded,
@@ -34,51 +81,46 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict
                                                              float* __restrict__ scales) {
   __shared__ uint32_t warp_max[32];
   const long long row = blockIdx.x;
+  const int lane = threadIdx.x & 31;
   const T* src = x + row * dim;
-  Raw8<T> raw[kChunks];
-  uint32_t top = 0;  // bits of |x|: ordered like the values, with NaN above infinity
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    raw[i] = load8<T, kVec>(src, (threadIdx.x + i * blockDim.x) * 8, dim);
-    float f[8];
-    unpack(raw[i], f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+  // lane s knows place s; a place outside the result is -1
+  long long place = -1;
+  if (lane < k) {
+    place = dst ? dst[row * k + lane] : row;
+    if (place >= out_rows) place = -1;
   }
+  Raw8<T> raw[kChunks];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) raw[i] = load8<T, kVec>(src, (threadIdx.x + i * blockDim.x) * 8, dim);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) top = max(top, top_bits(raw[i]));
   top = __reduce_max_sync(0xffffffffu, top);
   if (blockDim.x > 32) {
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
+    if (lane == 0) warp_max[threadIdx.x >> 5] = top;
     __syncthreads();
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    top = __reduce_max_sync(0xffffffffu, lane < warps ? warp_max[lane] : 0u);
+    top = __reduce_max_sync(0xffffffffu, lane < (blockDim.x >> 5) ? warp_max[lane] : 0u);
   }
   const bool finite = top < 0x7f800000u;
   const float scale = finite ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7fffffffu);
+  const bool tiny = scale < 0x1p-126f;
+  const float inv = __frcp_rn(scale);
   const bool codes = finite && scale > 0.f;
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     const int col = (threadIdx.x + i * blockDim.x) * 8;
-    if (col >= dim_padded) break;
-    float f[8];
-    unpack(raw[i], f);
-    uint32_t w[2] = {0, 0};
+    uint2 w = make_uint2(0, 0);
     if (codes) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = max(-127, min(127, __float2int_rn(__fdiv_rn(f[j], scale))));
-        w[j >> 2] |= static_cast<uint32_t>(c & 0xff) << (8 * (j & 3));
-      }
+      float f[8];
+      unpack(raw[i], f);
+      w = quantize8(f, scale, inv, tiny);
     }
     for (int s = 0; s < k; ++s) {
-      const long long pos = dst ? dst[row * k + s] : row;
-      if (pos >= 0 && pos < out_rows)
-        *reinterpret_cast<uint2*>(q + pos * dim_padded + col) = make_uint2(w[0], w[1]);
+      const long long pos = __shfl_sync(0xffffffffu, place, s);
+      if (pos >= 0 && col < dim_padded) *reinterpret_cast<uint2*>(q + pos * dim_padded + col) = w;
     }
   }
-  if (threadIdx.x < k) {
-    const long long pos = dst ? dst[row * k + threadIdx.x] : row;
-    if (pos >= 0 && pos < out_rows) scales[pos] = scale;
-  }
+  if (threadIdx.x < k && place >= 0) scales[place] = scale;
 }
 
 template <typename T, bool kVec>

@@ -255,6 +255,24 @@ def test_quantize_rows(T, dim, dtype):
     assert ((back - x.double()).abs() <= want_scale.double()[:, None] * (0.5 + 128 * H)).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_quantize_rows_next_to_halves(dtype):
+    """Values at, and one step of fp32 around, every half-way point between two codes, for several scales."""
+    from gmm_b200.int8 import quantize_rows
+    halves = torch.arange(-127, 127).float() + 0.5
+    rows = []
+    for top in (127.0, 1.0, 126.99999, 3.3e-30, 0.7, 2.0 ** -118, 2.0 ** -130):
+        scale = torch.tensor(top) / torch.tensor(127.0)
+        mid = halves * scale
+        for v in (mid, torch.nextafter(mid, torch.tensor(float("inf"))), torch.nextafter(mid, torch.tensor(float("-inf")))):
+            rows.append(torch.cat([torch.tensor([top]), v]))
+    x = torch.stack(rows).to(dtype)
+    x = x[torch.isfinite(x).all(1)]
+    q, scale = quantize_rows(x.cuda())
+    want_q, want_scale = spec_quantize(x)
+    assert torch.equal(scale.cpu(), want_scale) and torch.equal(q.cpu(), want_q)
+
+
 def test_quantize_rows_unaligned_and_strided():
     from gmm_b200.int8 import quantize_rows
     base = rows_of(13, 520, torch.bfloat16, seed=4).cuda()
