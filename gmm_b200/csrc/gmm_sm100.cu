@@ -1973,9 +1973,10 @@ int gmm_sm100_device_error(int* status_out, int clear) {
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyToSymbol(g_device_error)");
   }
-  int norm = 0;
+  int norm = 0, quant = 0;
   if (int rc = norm_device_error(&norm, clear != 0)) return rc;
-  if (status_out) *status_out = v ? v : norm;
+  if (int rc = quant_device_error(&quant, clear != 0)) return rc;
+  if (status_out) *status_out = v ? v : (norm ? norm : quant);
   return GMM_OK;
 }
 

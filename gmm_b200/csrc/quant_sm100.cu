@@ -12,12 +12,14 @@
 //
 // Bound by HBM: a row is read once (one block holds it in registers between
 // its maximum and its codes) and written k times, where a quantiser followed
-// by a gather would read and write the codes once more.
+// by a gather would read and write the codes once more.  Rows come through a
+// shared-memory ring and leave as one bulk store a place.
 
 #include <algorithm>
 #include <cstdio>
 
 #include "gmm_sm100.h"
+#include "row_ring.cuh"
 #include "row_vec.cuh"
 #include "status.h"
 
@@ -25,6 +27,7 @@ namespace gmm_sm100 {
 namespace {
 
 constexpr int kMaxDim = 65536;
+constexpr int kMaxRingDim = 16384;  // wider rows go through quantize_rows_kernel
 
 // Largest |x| of eight elements, as its fp32 bits: ordered like the values,
 // with NaN above infinity.  16-bit types compare two at a time.
@@ -73,72 +76,177 @@ __device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale, flo
                     __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }
 
-// One block per row; thread t holds the 8-element chunks t, t + blockDim.x, ...
-template <typename T, int kChunks, bool kVec>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, int dim, int dim_padded,
-                                                             const int32_t* __restrict__ dst, int k,
-                                                             long long out_rows, int8_t* __restrict__ q,
-                                                             float* __restrict__ scales) {
-  __shared__ uint32_t warp_max[32];
-  const long long row = blockIdx.x;
+struct QuantParams {
+  const void* x;
+  const int32_t* dst;
+  int8_t* q;
+  float* scales;
+  long long rows, out_rows;
+  int dim, dim_padded, k;
+};
+
+// Place `s` of a row for lane s of a warp; -1: none, or outside the result.
+__device__ __forceinline__ long long place_of(const QuantParams& p, long long row, int lane) {
+  if (lane >= p.k || row >= p.rows) return -1;
+  const long long place = p.dst ? p.dst[row * p.k + lane] : row;
+  return place < p.out_rows ? place : -1;
+}
+
+// What a row's codes are made with, from the largest |x| of each thread.
+struct RowScale {
+  float scale, inv;
+  bool codes, divide;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top, uint32_t* warp_max) {
   const int lane = threadIdx.x & 31;
-  const T* src = x + row * dim;
-  // lane s knows place s; a place outside the result is -1
-  long long place = -1;
-  if (lane < k) {
-    place = dst ? dst[row * k + lane] : row;
-    if (place >= out_rows) place = -1;
-  }
-  Raw8<T> raw[kChunks];
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) raw[i] = load8<T, kVec>(src, (threadIdx.x + i * blockDim.x) * 8, dim);
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kChunks; ++i) top = max(top, top_bits(raw[i]));
   top = __reduce_max_sync(0xffffffffu, top);
   if (blockDim.x > 32) {
     if (lane == 0) warp_max[threadIdx.x >> 5] = top;
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, lane < (blockDim.x >> 5) ? warp_max[lane] : 0u);
   }
+  RowScale r;
   const bool finite = top < 0x7f800000u;
-  const float scale = finite ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7fffffffu);
-  const bool tiny = scale < 0x1p-126f;
-  const float inv = __frcp_rn(scale);
-  const bool codes = finite && scale > 0.f;
+  r.scale = finite ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7fffffffu);
+  r.inv = __frcp_rn(r.scale);
+  r.divide = r.scale < 0x1p-126f;  // the reciprocal may not be finite
+  r.codes = finite && r.scale > 0.f;
+  return r;
+}
+
+// Eight elements of a row in the ring; kVec: on 16-byte boundaries.
+template <typename T, bool kVec>
+__device__ __forceinline__ Raw8<T> ring8(const uint8_t* row, int col, int dim) {
+  return load8<T, kVec>(reinterpret_cast<const T*>(row), col, dim);
+}
+
+// Persistent blocks over the ring.  A row's codes are staged in shared memory
+// (two buffers) and lane s of warp 0 stores them to place s.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(1024) quantize_ring_kernel(const QuantParams p, int slots) {
+  constexpr int kChunks = 2;  // 8-element chunks of a row a thread holds
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t warp_max[2][32];
+  uint8_t* staged = smem;  // 2 rows of codes
+  RowRing<1, kVec> ring;
+  ring.src[0] = static_cast<const char*>(p.x);
+  ring.bytes[0] = p.dim * sizeof(T);
+  ring.start(smem + 2 * p.dim_padded, slots, p.rows);
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  long long place = threadIdx.x < 32 ? place_of(p, blockIdx.x, lane) : -1;
+  int slot = 0, odd = 0;
+  uint32_t phase = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    ring.wait(slot, phase, row);
+    const uint8_t* in = ring.get(slot, 0, row);
+    Raw8<T> raw[kChunks];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      raw[i] = ring8<T, kVec>(in, (threadIdx.x + i * blockDim.x) * 8, p.dim);
+      top = max(top, top_bits(raw[i]));
+    }
+    // the stores that read this staging buffer two rows ago are done with it
+    if (threadIdx.x < 32) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    const RowScale rs = row_scale(top, warp_max[odd]);
+    if (blockDim.x == 32) __syncwarp();
+    if (threadIdx.x == 0 && !ring.dead) {  // every thread holds its part of the row
+      const long long next = row + static_cast<long long>(slots) * gridDim.x;
+      if (next < p.rows) ring.fetch(slot, next);
+    }
+    uint8_t* codes = staged + odd * p.dim_padded;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int col = (threadIdx.x + i * blockDim.x) * 8;
+      uint2 w = make_uint2(0, 0);
+      if (rs.codes) {
+        float f[8];
+        unpack(raw[i], f);
+        w = quantize8(f, rs.scale, rs.inv, rs.divide);
+      }
+      if (col < p.dim_padded) *reinterpret_cast<uint2*>(codes + col) = w;
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      if (place >= 0) {
+        p.scales[place] = rs.scale;
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.q + place * p.dim_padded),
+                     "r"(smem_u32(codes)), "r"(p.dim_padded)
+                     : "memory");
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      place = place_of(p, row + gridDim.x, lane);
+    }
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1;
+    }
+    odd ^= 1;
+  }
+  if (threadIdx.x < 32) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
+// Rows too wide for the ring, one block each; thread t holds the 8-element
+// chunks t, t + blockDim.x, ...
+template <typename T, int kChunks, bool kVec>
+__global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantParams p) {
+  __shared__ uint32_t warp_max[32];
+  const long long row = blockIdx.x;
+  const T* src = static_cast<const T*>(p.x) + row * p.dim;
+  const long long place = place_of(p, row, threadIdx.x & 31);
+  Raw8<T> raw[kChunks];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) raw[i] = load8<T, kVec>(src, (threadIdx.x + i * blockDim.x) * 8, p.dim);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) top = max(top, top_bits(raw[i]));
+  const RowScale rs = row_scale(top, warp_max);
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) {
     const int col = (threadIdx.x + i * blockDim.x) * 8;
     uint2 w = make_uint2(0, 0);
-    if (codes) {
+    if (rs.codes) {
       float f[8];
       unpack(raw[i], f);
-      w = quantize8(f, scale, inv, tiny);
+      w = quantize8(f, rs.scale, rs.inv, rs.divide);
     }
-    for (int s = 0; s < k; ++s) {
+    for (int s = 0; s < p.k; ++s) {
       const long long pos = __shfl_sync(0xffffffffu, place, s);
-      if (pos >= 0 && col < dim_padded) *reinterpret_cast<uint2*>(q + pos * dim_padded + col) = w;
+      if (pos >= 0 && col < p.dim_padded) *reinterpret_cast<uint2*>(p.q + pos * p.dim_padded + col) = w;
     }
   }
-  if (threadIdx.x < k && place >= 0) scales[place] = scale;
+  if (threadIdx.x < p.k && place >= 0) p.scales[place] = rs.scale;
 }
 
 template <typename T, bool kVec>
-void launch(const void* x, long long rows, int dim, int dim_padded, const int32_t* dst, int k, long long out_rows,
-            int8_t* q, float* scales, cudaStream_t s) {
-  const int chunks = dim_padded / 8;
-  const T* xt = static_cast<const T*>(x);
-  const unsigned grid = static_cast<unsigned>(rows);
-  auto threads = [&](int per) { return std::max(32, (chunks + 32 * per - 1) / (32 * per) * 32); };
-  if (chunks <= 256)
-    quantize_rows_kernel<T, 1, kVec><<<grid, threads(1), 0, s>>>(xt, dim, dim_padded, dst, k, out_rows, q, scales);
-  else if (chunks <= 2048)
-    quantize_rows_kernel<T, 2, kVec><<<grid, threads(2), 0, s>>>(xt, dim, dim_padded, dst, k, out_rows, q, scales);
-  else
-    quantize_rows_kernel<T, 8, kVec><<<grid, threads(8), 0, s>>>(xt, dim, dim_padded, dst, k, out_rows, q, scales);
+cudaError_t launch(const QuantParams& p, int sms, cudaStream_t s) {
+  const int chunks = p.dim_padded / 8;
+  if (p.dim <= kMaxRingDim && p.dim > 0) {
+    // As many blocks as threads and shared memory allow with two slots each,
+    // and up to four slots in what is left (two fit at every width).
+    const int threads = threads_for((chunks + 1) / 2);
+    const int slot = static_cast<int>(row_pitch(p.dim * sizeof(T), kVec)) + 8, fixed = 2 * p.dim_padded + 1024 + 512;
+    const int resident = std::max(1, std::min({16, 1024 / threads, kRingBytes / (fixed + 2 * slot)}));
+    const int slots = std::max(2, std::min(4, (kRingBytes / resident - fixed) / slot));
+    static std::atomic<unsigned long long> done{0};
+    auto kernel = quantize_ring_kernel<T, kVec>;
+    const cudaError_t e = allow_smem(kernel, done);
+    if (e != cudaSuccess) return e;
+    const int grid = static_cast<int>(std::min<long long>(p.rows, static_cast<long long>(sms) * resident));
+    kernel<<<grid, threads, 2 * p.dim_padded + slots * slot, s>>>(p, slots);
+    return cudaSuccess;
+  }
+  const unsigned grid = static_cast<unsigned>(p.rows);
+  quantize_rows_kernel<T, 8, kVec><<<grid, threads_for((chunks + 7) / 8), 0, s>>>(p);
+  return cudaSuccess;
 }
 
 }  // namespace
+
+int quant_device_error(int* status, bool clear) { return read_row_error(status, clear); }
+
 }  // namespace gmm_sm100
 
 extern "C" int gmm_sm100_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t dim,
@@ -164,16 +272,15 @@ extern "C" int gmm_sm100_quantize_rows(const void* x, int dtype, int64_t num_row
   if (int rc = current_sm_count(&sms)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int D = static_cast<int>(dim), P = (D + 15) / 16 * 16;
+  const QuantParams p{x, dst_pos, q, scale, num_rows, out_rows, D, P, k};
   const bool vec = D % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
   auto go = [&](auto t) {
     using T = decltype(t);
-    vec ? launch<T, true>(x, num_rows, D, P, dst_pos, k, out_rows, q, scale, s)
-        : launch<T, false>(x, num_rows, D, P, dst_pos, k, out_rows, q, scale, s);
+    const cudaError_t e = vec ? launch<T, true>(p, sms, s) : launch<T, false>(p, sms, s);
+    return e == cudaSuccess ? cudaGetLastError() : e;
   };
-  if (dtype == GMM_DTYPE_F32) go(float{});
-  else if (dtype == GMM_DTYPE_BF16) go(__nv_bfloat16{});
-  else go(__half{});
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
-  return GMM_OK;
+  const cudaError_t e = dtype == GMM_DTYPE_F32    ? go(float{})
+                        : dtype == GMM_DTYPE_BF16 ? go(__nv_bfloat16{})
+                                                  : go(__half{});
+  return e == cudaSuccess ? GMM_OK : set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -10,7 +10,8 @@ int set_error(int code, const char* msg) noexcept;
 // SM count of the current device; a status if it is not a B200-class GPU.
 int current_sm_count(int* sms);
 
-// The norm kernels' part of gmm_sm100_device_error.
+// The norm and quantiser kernels' parts of gmm_sm100_device_error.
 int norm_device_error(int* status, bool clear);
+int quant_device_error(int* status, bool clear);
 
 }  // namespace gmm_sm100
