@@ -17,9 +17,10 @@
 //   dw = sum_rows s act(g) dx yh,  dv = sum_rows dh xh,  dg = s act'(g) n dx
 // x' is computed again from y and x in fp32 (the same bytes as reading it
 // back, and without its rounding).  mean(t yh) needs dx, which needs
-// mean(u xh); it is linear in it, so three sums of one pass give both:
-//   C = sum u xh,  A = sum P e,  B = sum P r(x') xh   with e = dx' + r(x') u and
-//   P = s act(g) n:   sum t yh = A - (C / D) B.
+// mean(u xh); it is linear in it, so four sums of one pass give both.  With
+// Q = s act(g) (w + o) y:
+//   C = sum u x',  A1 = sum Q dx',  A2 = sum Q u,  B = sum Q x'
+//   c = r(x')^2 C / D,   sum t yh = r(y) (A1 + r(x') A2 - c r(x') B).
 // Everything is held in fp32 and rounded once, on store.  Rows are walked by
 // blocks in a fixed order and parameter gradients added up per block, then
 // over blocks in order, so results do not change from run to run.
@@ -27,7 +28,9 @@
 // Bound by HBM: a row is read once and written once.  The kernels stream
 // rows into shared memory with bulk copies (no registers and no threads held
 // by loads in flight), several rows ahead of the two block-wide sums a row
-// waits for; parameters stay in registers over all rows of a block.
+// waits for; parameters stay in registers over all rows of a block.  Next to
+// HBM comes the issue rate: two neighbouring elements share an instruction
+// (f32x2), and the sums of a row take half the shuffles of separate ones.
 
 #include <algorithm>
 #include <cstdio>
@@ -80,27 +83,66 @@ __device__ __forceinline__ float act_slope(float a, int act) {
   return act == GMM_GATE_TANH ? 1.f - a * a : act == GMM_GATE_SIGMOID ? a * (1.f - a) : 1.f;
 }
 
-// Sums of n values over the block; every thread gets them.  `scratch` holds
-// 32 * n floats; two calls in a row need different scratch.
-template <int n>
-__device__ __forceinline__ void block_sum(float (&s)[n], float* scratch) {
+// Two fp32 operations in one instruction, each rounded like its own.
+__device__ __forceinline__ void fma2(float* d, const float* a, const float* b, const float* c) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d[0]), "=f"(d[1])
+      : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+}
+__device__ __forceinline__ void mul2(float* d, const float* a, const float* b) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d[0]), "=f"(d[1])
+      : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+// A number for both halves.
+struct Both {
+  float v[2];
+  __device__ __forceinline__ explicit Both(float f) : v{f, f} {}
+  __device__ __forceinline__ operator const float*() const { return v; }
+};
+
+constexpr int kMaxWarps = 32;
+
+// Sum over the block; every thread gets it.  `scratch` holds kMaxWarps floats,
+// zero where there is no warp; two calls in a row need different scratch.
+__device__ __forceinline__ float block_sum(float s, float* scratch) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (blockDim.x == 32) return s;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) scratch[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = scratch[lane & 7] + scratch[8 + (lane & 7)];
+  if (blockDim.x > 16 * 32) s += scratch[16 + (lane & 7)] + scratch[24 + (lane & 7)];
 #pragma unroll
-    for (int j = 0; j < n; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-  if (blockDim.x > 32) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (lane == 0)
+  for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// Four sums over at most 16 warps.  Halves of a warp trade sums until each
+// group of eight lanes works on one: 9 shuffles in a warp instead of 20.
+// `scratch` holds 4 * 16 floats, zero where there is no warp.
+__device__ __forceinline__ void block_sum4(float (&s)[4], float* scratch) {
+  const int lane = threadIdx.x & 31;
+  const bool up = lane & 16, odd = lane & 8;
+  float a = up ? s[2] : s[0], b = up ? s[3] : s[1];
+  a += __shfl_xor_sync(0xffffffffu, up ? s[0] : s[2], 16);
+  b += __shfl_xor_sync(0xffffffffu, up ? s[1] : s[3], 16);
+  float t = odd ? b : a;
+  t += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
 #pragma unroll
-      for (int j = 0; j < n; ++j) scratch[j * 32 + warp] = s[j];
+  for (int o = 4; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (blockDim.x > 32) {  // lanes 8 j .. 8 j + 7 hold sum j of the warp
+    if ((lane & 7) == 0) scratch[(lane >> 3) * 16 + (threadIdx.x >> 5)] = t;
     __syncthreads();
+    t = scratch[(lane >> 3) * 16 + (lane & 7)] + scratch[(lane >> 3) * 16 + 8 + (lane & 7)];
 #pragma unroll
-    for (int j = 0; j < n; ++j) s[j] = lane < warps ? scratch[j * 32 + lane] : 0.f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-#pragma unroll
-      for (int j = 0; j < n; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+    for (int o = 4; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] = __shfl_sync(0xffffffffu, t, 8 * j);
 }
 
 // act(g) of a token gate's row, 1 for the others.
@@ -228,7 +270,7 @@ template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const NormParams p, int slots) {
   constexpr int kUnits = kE / V;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float scratch[2][2][32];  // by sum and by parity of the row
+  __shared__ float scratch[2][2][kMaxWarps];  // by sum and by parity of the row
   const int D = p.dim;
   RowRing<3, (V > 1)> ring;
   ring.src[0] = static_cast<const char*>(p.x);
@@ -238,6 +280,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
   ring.bytes[1] = kMode == kPreNorm ? 0 : D * sizeof(T);
   ring.bytes[2] = kMode == kFullGate ? D * (p.gate_f32 ? 4 : static_cast<int>(sizeof(T))) : 0;
   ring.start(smem, slots, p.rows);
+  if (threadIdx.x < 32)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scratch[i >> 1][i & 1][threadIdx.x] = 0.f;
 
   const int units = D / V;
   float pw[kE], vo[kE];
@@ -251,9 +296,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
     ring.wait(slot, phase, row);
-    const auto* xs = reinterpret_cast<const RawUnit<T, V>*>(ring.get(slot, 0, row));
+    const auto* xs = reinterpret_cast<const RawUnit<T, V>*>(smem + ring.at(slot, 0, row));
     float x[kE];
-    float sq[1] = {0.f};
+    float sq[2] = {0.f, 0.f};
     if constexpr (kMode == kPreNorm) {
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
@@ -261,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
         read_unit_or_0<T, V>(xs, c, c < units, x + i * V);
       }
     } else {
-      const uint8_t* ys = ring.get(slot, 1, row);
+      const auto* ys = smem + ring.at(slot, 1, row);
       float y[kE];
       RawUnit<T, V> xr[kUnits];
 #pragma unroll
@@ -270,45 +315,55 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
         read_unit_or_0<T, V>(ys, c, c < units, y + i * V);
         xr[i] = RawUnit<T, V>{};
         if (c < units) xr[i] = xs[c];
+      }
 #pragma unroll
-        for (int j = 0; j < V; ++j) sq[0] = fmaf(y[i * V + j], y[i * V + j], sq[0]);
-        if constexpr (kMode == kFullGate) {  // y * act(g): the gate is not needed again
+      for (int j = 0; j < kE; j += 2) fma2(sq, y + j, y + j, sq);
+      if constexpr (kMode == kFullGate) {  // y * act(g): the gate is not needed again
+        const auto* gs = smem + ring.at(slot, 2, row);
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int c = threadIdx.x + i * blockDim.x;
           float g[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) g[j] = 0.f;
-          if (c < units) read_param<T, V>(ring.get(slot, 2, row), p.gate_f32, c, g);
+          if (c < units) read_param<T, V>(gs, p.gate_f32, c, g);
 #pragma unroll
           for (int j = 0; j < V; ++j) y[i * V + j] *= act_of(g[j], p.act);
         }
       }
-      block_sum(sq, scratch[0][odd]);
-      const float ry = rsqrtf(sq[0] * inv_d + p.eps);
+      const float ry = rsqrtf(block_sum(sq[0] + sq[1], scratch[0][odd]) * inv_d + p.eps);
       if (p.rstd_y && threadIdx.x == 0) p.rstd_y[row] = ry;
-      const float c0 = ry * tok;
+      const Both c0(ry * tok);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) unpack_unit<T, V>(xr[i], x + i * V);
+#pragma unroll
+      for (int j = 0; j < kE; j += 2) {
+        mul2(y + j, y + j, c0);
+        fma2(x + j, y + j, pw + j, x + j);
+      }
       T* xn = static_cast<T*>(p.xn) + row * D;
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-        unpack_unit<T, V>(xr[i], x + i * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          x[i * V + j] = fmaf(y[i * V + j] * c0, pw[i * V + j], x[i * V + j]);
         if (c < units) write_unit<T, V>(xn, c, x + i * V);
       }
     }
     if (p.h) {
-      sq[0] = 0.f;
+      sq[0] = sq[1] = 0.f;
 #pragma unroll
-      for (int j = 0; j < kE; ++j) sq[0] = fmaf(x[j], x[j], sq[0]);
-      block_sum(sq, scratch[1][odd]);
-      const float rx = rsqrtf(sq[0] * inv_d + p.eps);
+      for (int j = 0; j < kE; j += 2) fma2(sq, x + j, x + j, sq);
+      const float rx = rsqrtf(block_sum(sq[0] + sq[1], scratch[1][odd]) * inv_d + p.eps);
       if (p.rstd_x && threadIdx.x == 0) p.rstd_x[row] = rx;
+      const Both r2(rx);
+#pragma unroll
+      for (int j = 0; j < kE; j += 2) {
+        mul2(x + j, x + j, r2);
+        mul2(x + j, x + j, vo + j);
+      }
       T* h = static_cast<T*>(p.h) + row * D;
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[i * V + j] *= rx * vo[i * V + j];
         if (c < units) write_unit<T, V>(h, c, x + i * V);
       }
     }
@@ -332,9 +387,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 // a single slot, behind a barrier of its own.
 template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const NormParams p, int slots) {
-  constexpr int kUnits = kE / V;
+  // A thread works on groups of kG elements: one unit, or two of one element.
+  constexpr int kU = V == 1 ? 2 : 1, kG = V * kU, kGroups = kE / kG;
+  static_assert(kThreads <= 16 * 32, "block_sum4");
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float scratch[2][3 * 32];
+  __shared__ float scratch[2][4 * 16];
   const int D = p.dim;
   RowRing<5, (V > 1)> ring;
   ring.src[0] = static_cast<const char*>(p.x);
@@ -348,6 +405,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
   ring.bytes[3] = p.dh ? D * sizeof(T) : 0;
   ring.bytes[4] = kMode == kFullGate ? D * (p.gate_f32 ? 4 : static_cast<int>(sizeof(T))) : 0;
   ring.start(smem, slots, p.rows);
+  if (threadIdx.x < 32)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scratch[i >> 1][(i & 1) * 32 + threadIdx.x] = 0.f;
 
   const int units = D / V;
   float pw[kE], vo[kE], acc[kE], dv[kE];
@@ -365,112 +425,150 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
     const float rx = p.dh ? p.rstd_x[row] : 0.f;
     const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
     ring.wait(slot, phase, row);
-    const uint8_t *in_x = ring.get(slot, 0, row), *in_y = ring.get(slot, 1, row), *in_dx = ring.get(slot, 2, row),
-                  *in_dh = ring.get(slot, 3, row), *in_g = ring.get(slot, 4, row);
-    // yh, e = dx' + rx u, xh, act(g), dh of unit i
-    // (past the row's end: zeros, as its parameters are; a branch around each
-    // unit would keep single elements' loads from being in flight together)
-    auto read = [&](int i, int c, float (&yh)[V], float (&e)[V], float (&xh)[V], float (&a)[V], float (&dh)[V]) {
-      const bool in = V > 1 || c < units;
-      read_unit_or_0<T, V>(in_x, c, in, xh);
-      if constexpr (kMode != kPreNorm) {
-        read_unit_or_0<T, V>(in_y, c, in, yh);
+    const uint8_t *in_x = smem + ring.at(slot, 0, row), *in_y = smem + ring.at(slot, 1, row),
+                  *in_dx = smem + ring.at(slot, 2, row), *in_dh = smem + ring.at(slot, 3, row),
+                  *in_g = smem + ring.at(slot, 4, row);
+    auto unit = [&](int g, int u) { return static_cast<int>(threadIdx.x + (g * kU + u) * blockDim.x); };
+    const Both to_x(kMode == kFullGate ? ry : ry * tok);
+    // Of a group's elements: y, Q (times act(g) with a gate per element, which
+    // `a` returns), x', u = dh (v + o), dh.  Zeros past the row's end.
+    auto read = [&](int g, float (&y)[kG], float (&q)[kG], float (&a)[kG], float (&x)[kG], float (&u)[kG],
+                    float (&dh)[kG]) {
+#pragma unroll
+      for (int k = 0; k < kU; ++k) {
+        const int c = unit(g, k);
+        const bool in = V > 1 || c < units;
+        read_unit_or_0<T, V>(in_x, c, in, x + k * V);
+        if constexpr (kMode != kPreNorm) read_unit_or_0<T, V>(in_y, c, in, y + k * V);
+        if (p.dh) {
+          read_unit_or_0<T, V>(in_dh, c, in, dh + k * V);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) dh[k * V + j] = 0.f;
+        }
         if constexpr (kMode == kFullGate) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) a[j] = 0.f;
-          if (in) read_param<T, V>(in_g, p.gate_f32, c, a);
-        }
+          for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
+          if (in) read_param<T, V>(in_g, p.gate_f32, c, a + k * V);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          yh[j] *= ry;
-          a[j] = kMode == kFullGate ? act_of(a[j], p.act) : tok;
-          xh[j] = fmaf(a[j] * pw[i * V + j], yh[j], xh[j]);
+          for (int j = 0; j < V; ++j) a[k * V + j] = act_of(a[k * V + j], p.act);
         }
       }
-      if (p.dxn) read_unit_or_0<T, V>(in_dx, c, in, e);
-      else
 #pragma unroll
-        for (int j = 0; j < V; ++j) e[j] = 0.f;
-      if (p.dh) {
-        read_unit_or_0<T, V>(in_dh, c, in, dh);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          xh[j] *= rx;
-          e[j] = fmaf(rx * dh[j], vo[i * V + j], e[j]);
+      for (int j = 0; j < kG; j += 2) {
+        if constexpr (kMode != kPreNorm) {
+          mul2(q + j, y + j, pw + g * kG + j);
+          if constexpr (kMode == kFullGate) mul2(q + j, q + j, a + j);
+          fma2(x + j, q + j, to_x, x + j);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) xh[j] = dh[j] = 0.f;
+        mul2(u + j, dh + j, vo + g * kG + j);
       }
     };
-    float sums[3] = {0.f, 0.f, 0.f};  // C, A, B / r(x'); A and B without the row's own gate
+    auto read_dx = [&](int g, float (&d)[kG]) {
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (V > 1 && c >= units) continue;
-      float yh[V], e[V], xh[V], a[V], dh[V];
-      read(i, c, yh, e, xh, a, dh);
+      for (int k = 0; k < kU; ++k) {
+        const int c = unit(g, k);
+        if (p.dxn) {
+          read_unit_or_0<T, V>(in_dx, c, V > 1 || c < units, d + k * V);
+        } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        sums[0] = fmaf(dh[j] * vo[i * V + j], xh[j], sums[0]);
+          for (int j = 0; j < V; ++j) d[k * V + j] = 0.f;
+        }
+      }
+    };
+    float s2[4][2] = {};  // C, A1, A2, B: even and odd elements
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (V > 1 && unit(g, 0) >= units) continue;
+      float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG];
+      read(g, y, q, a, x, u, dh);
+      if constexpr (kMode != kPreNorm) read_dx(g, d);
+#pragma unroll
+      for (int j = 0; j < kG; j += 2) {
+        fma2(s2[0], u + j, x + j, s2[0]);
         if constexpr (kMode != kPreNorm) {
-          const float q = pw[i * V + j] * yh[j] * (kMode == kFullGate ? a[j] : 1.f);
-          sums[1] = fmaf(q, e[j], sums[1]);
-          sums[2] = fmaf(q, xh[j], sums[2]);
+          fma2(s2[1], q + j, d + j, s2[1]);
+          fma2(s2[2], q + j, u + j, s2[2]);
+          fma2(s2[3], q + j, x + j, s2[3]);
         }
       }
     }
-    block_sum(sums, scratch[odd]);
+    float s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = s2[j][0] + s2[j][1];
+    block_sum4(s, scratch[odd]);
     // Every thread is past the previous row's last read of its slot.
     if (threadIdx.x == 0 && slots > 1 && !ring.dead && row >= gridDim.x) {
       const long long next = row + static_cast<long long>(slots - 1) * gridDim.x;
       if (next < p.rows) ring.fetch(slot == 0 ? slots - 1 : slot - 1, next);
     }
-    const float c1 = rx * (sums[0] * inv_d);  // dx = e - c1 xh
-    const float qdx = sums[1] - c1 * sums[2];
-    const float m = qdx * inv_d * tok;        // mean(t yh)
+    const float cx = rx * rx * (s[0] * inv_d) * rx;       // dx = dx' + r(x') u - cx x'
+    const float qdx = ry * (s[1] + rx * s[2] - cx * s[3]);  // sum of s (w + o) yh [act(g)] dx
+    const float m = qdx * inv_d * tok;                    // mean(t yh)
     if (kMode == kSharedGate && p.gate_mode == kGateToken && threadIdx.x == 0) {
       const float d = qdx * act_slope(tok, p.act);
       if (p.gate_f32) static_cast<float*>(p.dgate_row)[row] = d;
       else static_cast<T*>(p.dgate_row)[row] = from_float<T>(d);
     }
+    const Both r2(rx), neg_cx(-cx), neg_m(-ry * ry * m), ry2(ry);
     T* dx_out = static_cast<T*>(p.dx) + row * D;
     T* dy_out = static_cast<T*>(p.dy) + row * D;
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (V > 1 && c >= units) continue;
-      const bool in = V > 1 || c < units;
-      float yh[V], e[V], xh[V], a[V], dh[V];
-      read(i, c, yh, e, xh, a, dh);
+    for (int g = 0; g < kGroups; ++g) {
+      if (V > 1 && unit(g, 0) >= units) continue;
+      float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG];
+      read(g, y, q, a, x, u, dh);
+      read_dx(g, d);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        e[j] = fmaf(-c1, xh[j], e[j]);  // dx
-        dv[i * V + j] = fmaf(dh[j], xh[j], dv[i * V + j]);
+      for (int j = 0; j < kG; j += 2) {
+        const int e = g * kG + j;
+        fma2(d + j, u + j, r2, d + j);
+        fma2(d + j, x + j, neg_cx, d + j);  // dx
+        mul2(x + j, x + j, r2);
+        fma2(dv + e, dh + j, x + j, dv + e);
       }
-      if (in) write_unit<T, V>(dx_out, c, e);
+#pragma unroll
+      for (int k = 0; k < kU; ++k) {
+        const int c = unit(g, k);
+        if (V > 1 || c < units) write_unit<T, V>(dx_out, c, d + k * V);
+      }
       if constexpr (kMode != kPreNorm) {
-        float dg[V];
+        float dg[kG];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float ad = a[j] * e[j];
-          acc[i * V + j] = fmaf(ad, yh[j], acc[i * V + j]);
-          if constexpr (kMode == kFullGate) dg[j] = pw[i * V + j] * yh[j] * e[j] * act_slope(a[j], p.act);
-          yh[j] = ry * fmaf(ad, pw[i * V + j], -yh[j] * m);  // dy
-        }
-        if (in) write_unit<T, V>(dy_out, c, yh);
-        if constexpr (kMode == kFullGate) {
-          if (!in) continue;
-          if (p.gate_f32 && sizeof(T) == 2) {
-            float* out = static_cast<float*>(p.dgate_row) + row * D;
-            if constexpr (V == 1) {
-              out[c] = dg[0];
-            } else {
+        for (int j = 0; j < kG; j += 2) {
+          const int e = g * kG + j;
+          if constexpr (kMode == kFullGate) {
+            float yh[2];
+            mul2(yh, y + j, ry2);
 #pragma unroll
-              for (int q = 0; q < V / 4; ++q) write_unit<float, 4>(out, c * (V / 4) + q, dg + 4 * q);
-            }
+            for (int i = 0; i < 2; ++i) dg[j + i] = pw[e + i] * yh[i] * d[j + i] * act_slope(a[j + i], p.act);
+            mul2(d + j, d + j, a + j);
+            fma2(acc + e, d + j, yh, acc + e);
+            mul2(d + j, d + j, ry2);
           } else {
-            write_unit<T, V>(static_cast<T*>(p.dgate_row) + row * D, c, dg);
+            mul2(d + j, d + j, to_x);
+            fma2(acc + e, d + j, y + j, acc + e);
+          }
+          mul2(y + j, y + j, neg_m);
+          fma2(y + j, d + j, pw + e, y + j);  // dy
+        }
+#pragma unroll
+        for (int k = 0; k < kU; ++k) {
+          const int c = unit(g, k);
+          if (V == 1 && c >= units) continue;
+          write_unit<T, V>(dy_out, c, y + k * V);
+          if constexpr (kMode == kFullGate) {
+            if (p.gate_f32 && sizeof(T) == 2) {
+              float* out = static_cast<float*>(p.dgate_row) + row * D;
+              if constexpr (V == 1) {
+                out[c] = dg[k];
+              } else {
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i) write_unit<float, 4>(out, c * (V / 4) + i, dg + 4 * i);
+              }
+            } else {
+              write_unit<T, V>(static_cast<T*>(p.dgate_row) + row * D, c, dg + k * V);
+            }
           }
         }
       }
@@ -491,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
   float* part = p.partial + static_cast<long long>(blockIdx.x) * D;
   const long long slice = static_cast<long long>(gridDim.x) * D;
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
+  for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c >= units) continue;
     if constexpr (V == 1) {
@@ -523,7 +621,9 @@ __device__ __forceinline__ float gate1(const NormParams& p, long long row, int c
 // owns elements threadIdx.x + i * blockDim.x, read from global memory.
 template <typename T, int kE>
 __global__ void __launch_bounds__(kMaxThreads) norm_bwd_kernel(const NormParams p) {
-  __shared__ float scratch[3 * 32];
+  __shared__ float scratch[4 * 16];
+  if (threadIdx.x < 64) scratch[threadIdx.x] = 0.f;
+  __syncthreads();
   const int D = p.dim;
   const float inv_d = 1.f / static_cast<float>(D);
   float acc[kE], dv[kE];
@@ -543,7 +643,8 @@ __global__ void __launch_bounds__(kMaxThreads) norm_bwd_kernel(const NormParams 
       yh[i] = in_row && p.y ? as_float(static_cast<const T*>(p.y)[at + col]) * ry : 0.f;
       e[i] = in_row && p.dxn ? as_float(static_cast<const T*>(p.dxn)[at + col]) : 0.f;
     }
-    float sums[3] = {0.f, 0.f, 0.f};  // C, A, B / r(x'); A and B without the row's own gate
+    // sum u xh, sum P e, sum P xh with P = s (w + o) yh [act(g)]; e = dx' + r(x') u
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kE; ++i) {
       const int col = threadIdx.x + i * blockDim.x;
@@ -566,7 +667,7 @@ __global__ void __launch_bounds__(kMaxThreads) norm_bwd_kernel(const NormParams 
       sums[1] = fmaf(q, e[i], sums[1]);
       sums[2] = fmaf(q, xh[i], sums[2]);
     }
-    block_sum(sums, scratch);
+    block_sum4(sums, scratch);
     const float c1 = rx * (sums[0] * inv_d);
     const float qdx = sums[1] - c1 * sums[2];
     const float m = qdx * inv_d * tok;

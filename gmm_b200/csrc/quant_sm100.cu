@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(1024) quantize_ring_kernel(const QuantParams p
   uint32_t phase = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     ring.wait(slot, phase, row);
-    const uint8_t* in = ring.get(slot, 0, row);
+    const uint8_t* in = smem + 2 * p.dim_padded + ring.at(slot, 0, row);
     Raw8<T> raw[kChunks];
     uint32_t top = 0;
 #pragma unroll

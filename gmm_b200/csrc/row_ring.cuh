@@ -127,13 +127,13 @@ struct RowRing {
     __syncthreads();
   }
 
-  // Input i of the row in `slot`.
-  __device__ __forceinline__ const uint8_t* get(int slot, int i, long long row) const {
-    uint32_t at = slot * slot_bytes;
+  // Where input i of the row in `slot` starts, from slot 0's start.
+  __device__ __forceinline__ uint32_t at(int slot, int i, long long row) const {
+    uint32_t off = slot * slot_bytes;
 #pragma unroll
-    for (int j = 0; j < i; ++j) at += pitch(j);
-    if (!kAligned) at += static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u);
-    return smem + at;
+    for (int j = 0; j < i; ++j) off += pitch(j);
+    if (!kAligned) off += static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u);
+    return off;
   }
 
   // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  The
