@@ -155,13 +155,24 @@ __device__ __forceinline__ float token_gate(const NormParams& p, long long row) 
 
 // ------------------------------------------------------------------ ring kernels
 // A thread owns kE elements of every row, in units of V neighbouring elements:
-// the units threadIdx.x + i * blockDim.x.  V is 16 bytes where every row
-// starts on a 16-byte boundary, else 1 (neighbouring threads then read
-// neighbouring elements).
+// the units threadIdx.x + i * blockDim.x.  Three layouts:
+//   kWhole    V is 16 bytes and rows are whole words;
+//   kShifted  V is 16 bytes and tensors start on a word but rows (dim not a
+//             multiple of V) do not.  Units are the words of memory, so that
+//             loads and stores stay whole; a row's first and last unit are
+//             partly its neighbours' and masked.  A row starts `shift` elements
+//             into its first unit; the grid is a multiple of the shift's
+//             period, so a block's rows all have the same one and its
+//             parameters and sums stay in registers;
+//   kSingle   V is 1 (tensors off the 16-byte grid): neighbouring threads read
+//             neighbouring elements.
+// 16384 x 4095 bf16, channel gate: kSingle 163 us forward, 623 forward and
+// backward; 4096 columns (kWhole) 88 and 231; kShifted, see the launches.
+enum Layout { kWhole = 0, kShifted = 1, kSingle = 2 };
 enum RingMode { kPreNorm = 0, kSharedGate = 1, kFullGate = 2 };  // no y | gate none, channel, token | gate per element
 
-template <typename T>
-constexpr int kV = 16 / static_cast<int>(sizeof(T));
+template <typename T, int kLayout>
+constexpr int kUnit = kLayout == kSingle ? 1 : 16 / static_cast<int>(sizeof(T));
 
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4& r, float* f) {
@@ -232,47 +243,88 @@ __device__ __forceinline__ void write_unit(T* row, int c, const float* f) {
   }
 }
 
+// Which of the row's elements a unit holds.
+template <int V, int kLayout>
+struct Span {
+  int dim, units, shift;
+  __device__ __forceinline__ Span(int d) : dim(d) {
+    shift = kLayout == kShifted ? static_cast<int>(static_cast<long long>(blockIdx.x) * d % V) : 0;
+    units = (shift + d + V - 1) / V;
+  }
+  __device__ __forceinline__ bool partial(int c) const { return kLayout == kShifted && (c == 0 || c == units - 1); }
+  __device__ __forceinline__ int col(int c, int j) const { return c * V + j - shift; }
+  __device__ __forceinline__ bool has(int c, int j) const { return col(c, j) >= 0 && col(c, j) < dim; }
+  // What a partial unit holds of other rows becomes 0.
+  __device__ __forceinline__ void mask(int c, float* f) const {
+    if (partial(c))
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = has(c, j) ? f[j] : 0.f;
+  }
+  // The same unit of a row in global memory: rows of one block start at the same place in a word.
+  template <typename T>
+  __device__ __forceinline__ void write(T* row, int c, const float* f) const {
+    if (partial(c)) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (has(c, j)) row[col(c, j)] = from_float<T>(f[j]);
+    } else {
+      write_unit<T, V>(row - shift, c, f);
+    }
+  }
+};
+
 // s (w + o), times act(g) of a channel gate; v + o.  Zero past the row's end.
 // All loads first: they come from DRAM, one latency for all of them.
-template <typename T, int V, int kE, int kMode>
-__device__ __forceinline__ void row_params(const NormParams& p, bool with_v, float (&pw)[kE], float (&vo)[kE]) {
-  const int units = p.dim / V;
+template <typename T, int V, int kLayout, int kE, int kMode>
+__device__ __forceinline__ void row_params(const NormParams& p, const Span<V, kLayout>& span, bool with_v,
+                                           float (&pw)[kE], float (&vo)[kE]) {
   const bool channel = kMode == kSharedGate && p.gate_mode == kGateChannel;
   float g[kMode == kSharedGate ? kE : 1];
+  auto load = [&](const void* row, int f32, int c, float* f) {
+    if constexpr (kLayout == kShifted) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (span.has(c, j)) read_param<T, 1>(row, f32, span.col(c, j), f + j);
+    } else {
+      if (c < span.units) read_param<T, V>(row, f32, c, f);
+    }
+  };
 #pragma unroll
   for (int j = 0; j < kE; ++j) pw[j] = vo[j] = 0.f;
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    if (kMode != kPreNorm && c < units) read_param<T, V>(p.w, p.w_f32, c, pw + i * V);
-    if (with_v && c < units) read_param<T, V>(p.v, p.w_f32, c, vo + i * V);
+    if (kMode != kPreNorm) load(p.w, p.w_f32, c, pw + i * V);
+    if (with_v) load(p.v, p.w_f32, c, vo + i * V);
     if constexpr (kMode == kSharedGate) {
 #pragma unroll
       for (int j = 0; j < V; ++j) g[i * V + j] = 0.f;
-      if (channel && c < units) read_param<T, V>(p.gate, p.gate_f32, c, g + i * V);
+      if (channel) load(p.gate, p.gate_f32, c, g + i * V);
     }
   }
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
-    const bool in = threadIdx.x + i * blockDim.x < units;
+    const int c = threadIdx.x + i * blockDim.x;
 #pragma unroll
-    for (int j = i * V; j < (i + 1) * V; ++j) {
+    for (int j = 0; j < V; ++j) {
+      const bool in = span.has(c, j);
+      const int e = i * V + j;
       if (kMode != kPreNorm) {
-        pw[j] = in ? (pw[j] + p.offset) * p.scale : 0.f;
-        if (kMode == kSharedGate && channel) pw[j] *= act_of(g[j], p.act);
+        pw[e] = in ? (pw[e] + p.offset) * p.scale : 0.f;
+        if (kMode == kSharedGate && channel) pw[e] *= act_of(g[e], p.act);
       }
-      vo[j] = in && with_v ? vo[j] + p.offset : 0.f;
+      vo[e] = in && with_v ? vo[e] + p.offset : 0.f;
     }
   }
 }
 
-template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
+template <typename T, int kLayout, int kE, int kMode, int kThreads, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const NormParams p, int slots) {
-  constexpr int kUnits = kE / V;
+  constexpr int V = kUnit<T, kLayout>, kUnits = kE / V;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float scratch[2][2][kMaxWarps];  // by sum and by parity of the row
   const int D = p.dim;
-  RowRing<3, (V > 1)> ring;
+  RowRing<3, kLayout == kWhole> ring;
   ring.src[0] = static_cast<const char*>(p.x);
   ring.src[1] = static_cast<const char*>(p.y);
   ring.src[2] = static_cast<const char*>(p.gate);
@@ -284,9 +336,15 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][i & 1][threadIdx.x] = 0.f;
 
-  const int units = D / V;
+  const Span<V, kLayout> span(D);
+  const int units = span.units;
   float pw[kE], vo[kE];
-  row_params<T, V, kE, kMode>(p, p.h != nullptr, pw, vo);
+  row_params<T, V, kLayout, kE, kMode>(p, span, p.h != nullptr, pw, vo);
+  auto input = [&](int i, int slot, long long row) {
+    return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
+  };
+  // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
+  const int gate_words = kLayout == kShifted && sizeof(T) == 2 && p.gate_f32 ? span.shift / 4 * 16 : 0;
   __syncthreads();  // barriers initialised
   const float inv_d = 1.f / static_cast<float>(D);
 
@@ -296,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
     ring.wait(slot, phase, row);
-    const auto* xs = reinterpret_cast<const RawUnit<T, V>*>(smem + ring.at(slot, 0, row));
+    const auto* xs = reinterpret_cast<const RawUnit<T, V>*>(input(0, slot, row));
     float x[kE];
     float sq[2] = {0.f, 0.f};
     if constexpr (kMode == kPreNorm) {
@@ -304,22 +362,24 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
         read_unit_or_0<T, V>(xs, c, c < units, x + i * V);
+        span.mask(c, x + i * V);
       }
     } else {
-      const auto* ys = smem + ring.at(slot, 1, row);
+      const auto* ys = input(1, slot, row);
       float y[kE];
       RawUnit<T, V> xr[kUnits];
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
         read_unit_or_0<T, V>(ys, c, c < units, y + i * V);
+        span.mask(c, y + i * V);
         xr[i] = RawUnit<T, V>{};
         if (c < units) xr[i] = xs[c];
       }
 #pragma unroll
       for (int j = 0; j < kE; j += 2) fma2(sq, y + j, y + j, sq);
       if constexpr (kMode == kFullGate) {  // y * act(g): the gate is not needed again
-        const auto* gs = smem + ring.at(slot, 2, row);
+        const auto* gs = input(2, slot, row) - gate_words;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
           const int c = threadIdx.x + i * blockDim.x;
@@ -327,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
           for (int j = 0; j < V; ++j) g[j] = 0.f;
           if (c < units) read_param<T, V>(gs, p.gate_f32, c, g);
+          span.mask(c, g);
 #pragma unroll
           for (int j = 0; j < V; ++j) y[i * V + j] *= act_of(g[j], p.act);
         }
@@ -335,7 +396,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
       if (p.rstd_y && threadIdx.x == 0) p.rstd_y[row] = ry;
       const Both c0(ry * tok);
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) unpack_unit<T, V>(xr[i], x + i * V);
+      for (int i = 0; i < kUnits; ++i) {
+        unpack_unit<T, V>(xr[i], x + i * V);
+        span.mask(threadIdx.x + i * blockDim.x, x + i * V);
+      }
 #pragma unroll
       for (int j = 0; j < kE; j += 2) {
         mul2(y + j, y + j, c0);
@@ -345,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-        if (c < units) write_unit<T, V>(xn, c, x + i * V);
+        if (c < units) span.write(xn, c, x + i * V);
       }
     }
     if (p.h) {
@@ -364,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-        if (c < units) write_unit<T, V>(h, c, x + i * V);
+        if (c < units) span.write(h, c, x + i * V);
       }
     }
     // Every thread has read the slot before the (first or only) sum's barrier.
@@ -385,15 +449,16 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 // (re-reading shared memory costs less than holding four rows in registers),
 // so a slot is refilled one row later, past the next row's barrier -- or, with
 // a single slot, behind a barrier of its own.
-template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
+template <typename T, int kLayout, int kE, int kMode, int kThreads, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const NormParams p, int slots) {
+  constexpr int V = kUnit<T, kLayout>;
   // A thread works on groups of kG elements: one unit, or two of one element.
   constexpr int kU = V == 1 ? 2 : 1, kG = V * kU, kGroups = kE / kG;
   static_assert(kThreads <= 16 * 32, "block_sum4");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float scratch[2][4 * 16];
   const int D = p.dim;
-  RowRing<5, (V > 1)> ring;
+  RowRing<5, kLayout == kWhole> ring;
   ring.src[0] = static_cast<const char*>(p.x);
   ring.src[1] = static_cast<const char*>(p.y);
   ring.src[2] = static_cast<const char*>(p.dxn);
@@ -409,9 +474,15 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][(i & 1) * 32 + threadIdx.x] = 0.f;
 
-  const int units = D / V;
+  const Span<V, kLayout> span(D);
+  const int units = span.units;
   float pw[kE], vo[kE], acc[kE], dv[kE];
-  row_params<T, V, kE, kMode>(p, p.dh != nullptr, pw, vo);
+  row_params<T, V, kLayout, kE, kMode>(p, span, p.dh != nullptr, pw, vo);
+  auto input = [&](int i, int slot, long long row) {
+    return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
+  };
+  // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
+  const int gate_words = kLayout == kShifted && sizeof(T) == 2 && p.gate_f32 ? span.shift / 4 * 16 : 0;
 #pragma unroll
   for (int j = 0; j < kE; ++j) acc[j] = dv[j] = 0.f;
   __syncthreads();  // barriers initialised
@@ -425,9 +496,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
     const float rx = p.dh ? p.rstd_x[row] : 0.f;
     const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
     ring.wait(slot, phase, row);
-    const uint8_t *in_x = smem + ring.at(slot, 0, row), *in_y = smem + ring.at(slot, 1, row),
-                  *in_dx = smem + ring.at(slot, 2, row), *in_dh = smem + ring.at(slot, 3, row),
-                  *in_g = smem + ring.at(slot, 4, row);
+    const uint8_t *in_x = input(0, slot, row), *in_y = input(1, slot, row), *in_dx = input(2, slot, row),
+                  *in_dh = input(3, slot, row), *in_g = input(4, slot, row) - gate_words;
     auto unit = [&](int g, int u) { return static_cast<int>(threadIdx.x + (g * kU + u) * blockDim.x); };
     const Both to_x(kMode == kFullGate ? ry : ry * tok);
     // Of a group's elements: y, Q (times act(g) with a gate per element, which
@@ -439,9 +509,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
         const int c = unit(g, k);
         const bool in = V > 1 || c < units;
         read_unit_or_0<T, V>(in_x, c, in, x + k * V);
-        if constexpr (kMode != kPreNorm) read_unit_or_0<T, V>(in_y, c, in, y + k * V);
+        span.mask(c, x + k * V);
+        if constexpr (kMode != kPreNorm) {
+          read_unit_or_0<T, V>(in_y, c, in, y + k * V);
+          span.mask(c, y + k * V);
+        }
         if (p.dh) {
           read_unit_or_0<T, V>(in_dh, c, in, dh + k * V);
+          span.mask(c, dh + k * V);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) dh[k * V + j] = 0.f;
@@ -450,6 +525,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
           if (in) read_param<T, V>(in_g, p.gate_f32, c, a + k * V);
+          span.mask(c, a + k * V);
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = act_of(a[k * V + j], p.act);
         }
@@ -470,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
         const int c = unit(g, k);
         if (p.dxn) {
           read_unit_or_0<T, V>(in_dx, c, V > 1 || c < units, d + k * V);
+          span.mask(c, d + k * V);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) d[k * V + j] = 0.f;
@@ -530,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
 #pragma unroll
       for (int k = 0; k < kU; ++k) {
         const int c = unit(g, k);
-        if (V > 1 || c < units) write_unit<T, V>(dx_out, c, d + k * V);
+        if (V > 1 || c < units) span.write(dx_out, c, d + k * V);
       }
       if constexpr (kMode != kPreNorm) {
         float dg[kG];
@@ -556,18 +633,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
         for (int k = 0; k < kU; ++k) {
           const int c = unit(g, k);
           if (V == 1 && c >= units) continue;
-          write_unit<T, V>(dy_out, c, y + k * V);
+          span.write(dy_out, c, y + k * V);
           if constexpr (kMode == kFullGate) {
             if (p.gate_f32 && sizeof(T) == 2) {
               float* out = static_cast<float*>(p.dgate_row) + row * D;
-              if constexpr (V == 1) {
-                out[c] = dg[k];
+              if (V == 1 || span.partial(c)) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                  if (span.has(c, j)) out[span.col(c, j)] = dg[k * V + j];
               } else {
 #pragma unroll
-                for (int i = 0; i < V / 4; ++i) write_unit<float, 4>(out, c * (V / 4) + i, dg + 4 * i);
+                for (int i = 0; i < V / 4; ++i)
+                  write_unit<float, 4>(out - span.shift, c * (V / 4) + i, dg + 4 * i);
               }
             } else {
-              write_unit<T, V>(static_cast<T*>(p.dgate_row) + row * D, c, dg + k * V);
+              span.write(static_cast<T*>(p.dgate_row) + row * D, c, dg + k * V);
             }
           }
         }
@@ -591,15 +671,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    if (c >= units) continue;
-    if constexpr (V == 1) {
-      if (kMode != kPreNorm) part[c] = acc[i];
-      if (p.dh) part[slice + c] = dv[i];
-    } else {
+    if (kLayout == kWhole && D % 4 == 0) {
+      if (c >= units) continue;
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) {
         if (kMode != kPreNorm) write_unit<float, 4>(part, c * (V / 4) + q, acc + i * V + 4 * q);
         if (p.dh) write_unit<float, 4>(part + slice, c * (V / 4) + q, dv + i * V + 4 * q);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (!span.has(c, j)) continue;
+        if (kMode != kPreNorm) part[span.col(c, j)] = acc[i * V + j];
+        if (p.dh) part[slice + span.col(c, j)] = dv[i * V + j];
       }
     }
   }
@@ -775,21 +859,41 @@ RingShape ring_shape(int dim, int per_thread, int max_threads_sm, size_t slot_by
   return r;
 }
 
-template <typename T, int V, int kE, int kMode, int kThreads, int kBlocks>
-cudaError_t launch_fwd_ring(const NormParams& p, const RingShape& r, int sms, cudaStream_t s) {
+// The layout of a call's rows, the elements a row's units span, and the number
+// of blocks after which rows start at the same place in a word again.
+struct RowLayout {
+  int layout, span, period;
+};
+RowLayout row_layout(int dim, int es, bool words) {
+  const int v = 16 / es;
+  if (!words) return {kSingle, dim, 1};
+  if (dim % v == 0) return {kWhole, dim, 1};
+  int period = v;
+  for (int d = dim; d % 2 == 0; d /= 2) period /= 2;
+  return {kShifted, dim + 2 * (v - 1), period};
+}
+
+// Blocks for `rows`: at most `most`, and with several rows a block a multiple of the period.
+int blocks_for(int64_t rows, int64_t most, int period) {
+  if (rows <= most) return static_cast<int>(rows);
+  return static_cast<int>(std::max<int64_t>(period, most / period * period));
+}
+
+template <typename T, int kLayout, int kE, int kMode, int kThreads, int kBlocks>
+cudaError_t launch_fwd_ring(const NormParams& p, const RingShape& r, int period, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = norm_fwd_ring_kernel<T, V, kE, kMode, kThreads, kBlocks>;
+  auto kernel = norm_fwd_ring_kernel<T, kLayout, kE, kMode, kThreads, kBlocks>;
   const cudaError_t e = allow_smem(kernel, done);
   if (e != cudaSuccess) return e;
-  const int grid = static_cast<int>(std::min<long long>(p.rows, static_cast<long long>(sms) * r.resident));
+  const int grid = blocks_for(p.rows, static_cast<int64_t>(sms) * r.resident, period);
   kernel<<<grid, r.threads, r.smem, s>>>(p, r.slots);
   return cudaSuccess;
 }
 
-template <typename T, int V, int kMode, int kThreads, int kBlocks>
+template <typename T, int kLayout, int kMode, int kThreads, int kBlocks>
 cudaError_t launch_bwd_ring(const NormParams& p, const RingShape& r, int blocks, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = norm_bwd_ring_kernel<T, V, 16, kMode, kThreads, kBlocks>;
+  auto kernel = norm_bwd_ring_kernel<T, kLayout, 16, kMode, kThreads, kBlocks>;
   const cudaError_t e = allow_smem(kernel, done);
   if (e != cudaSuccess) return e;
   kernel<<<blocks, r.threads, r.smem, s>>>(p, r.slots);
@@ -802,64 +906,86 @@ int mode_of(const NormParams& p) {
 
 // Bytes of a slot that holds `inputs` rows of the data type and, with a gate
 // per element, one of the gate's.
-size_t slot_bytes(const NormParams& p, int es, bool vec, int inputs) {
+size_t slot_bytes(const NormParams& p, int es, int layout, int inputs) {
+  const bool whole = layout == kWhole;
   const uint32_t gate = p.gate_mode == GMM_GATE_MODE_FULL ? p.dim * (p.gate_f32 ? 4 : es) : 0;
-  return static_cast<size_t>(row_pitch(p.dim * es, vec)) * inputs + (gate ? row_pitch(gate, vec) : 0);
+  return static_cast<size_t>(row_pitch(p.dim * es, whole)) * inputs + (gate ? row_pitch(gate, whole) : 0);
 }
 
-template <typename T, int V, int kE, int kThreads, int kBlocks>
-cudaError_t fwd_ring_mode(const NormParams& p, int sms, cudaStream_t s) {
-  const RingShape r = ring_shape(p.dim, kE, kThreads * kBlocks, slot_bytes(p, sizeof(T), V > 1, p.y ? 2 : 1));
+template <typename T, int kLayout, int kE, int kThreads, int kBlocks>
+cudaError_t fwd_ring_mode(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
+  const RingShape r = ring_shape(l.span, kE, kThreads * kBlocks, slot_bytes(p, sizeof(T), kLayout, p.y ? 2 : 1));
   switch (mode_of(p)) {
-    case kPreNorm: return launch_fwd_ring<T, V, kE, kPreNorm, kThreads, kBlocks>(p, r, sms, s);
-    case kSharedGate: return launch_fwd_ring<T, V, kE, kSharedGate, kThreads, kBlocks>(p, r, sms, s);
-    default: return launch_fwd_ring<T, V, kE, kFullGate, kThreads, kBlocks>(p, r, sms, s);
+    case kPreNorm: return launch_fwd_ring<T, kLayout, kE, kPreNorm, kThreads, kBlocks>(p, r, l.period, sms, s);
+    case kSharedGate: return launch_fwd_ring<T, kLayout, kE, kSharedGate, kThreads, kBlocks>(p, r, l.period, sms, s);
+    default: return launch_fwd_ring<T, kLayout, kE, kFullGate, kThreads, kBlocks>(p, r, l.period, sms, s);
   }
 }
 
-template <typename T, int V>
-cudaError_t fwd_ring_width(const NormParams& p, int sms, cudaStream_t s) {
-  if (p.dim <= 4096) return fwd_ring_mode<T, V, 8, 512, 2>(p, sms, s);
-  if (p.dim <= 8192) return fwd_ring_mode<T, V, 8, 1024, 1>(p, sms, s);
-  return fwd_ring_mode<T, V, 16, 1024, 1>(p, sms, s);
+template <typename T, int kLayout>
+cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
+  if (l.span <= 4096) return fwd_ring_mode<T, kLayout, 8, 512, 2>(p, l, sms, s);
+  if (l.span <= 8192) return fwd_ring_mode<T, kLayout, 8, 1024, 1>(p, l, sms, s);
+  return fwd_ring_mode<T, kLayout, 16, 1024, 1>(p, l, sms, s);
 }
 
+constexpr int kMaxRingFwdSpan = 16384;
+
 template <typename T>
-cudaError_t launch_fwd(const NormParams& p, bool vec, int sms, cudaStream_t s) {
-  return vec ? fwd_ring_width<T, kV<T>>(p, sms, s) : fwd_ring_width<T, 1>(p, sms, s);
+cudaError_t launch_fwd(const NormParams& p, bool words, int sms, cudaStream_t s) {
+  RowLayout l = row_layout(p.dim, sizeof(T), words);
+  if (l.span > kMaxRingFwdSpan) l = row_layout(p.dim, sizeof(T), false);
+  switch (l.layout) {
+    case kWhole: return fwd_ring_width<T, kWhole>(p, l, sms, s);
+    case kShifted: return fwd_ring_width<T, kShifted>(p, l, sms, s);
+    default: return fwd_ring_width<T, kSingle>(p, l, sms, s);
+  }
 }
 
 // The ring's backward kernels keep 16 elements a thread (their parameters and
 // sums over rows in registers) in at most 512 threads.
-constexpr int kMaxRingBwdDim = 8192;
+constexpr int kMaxRingBwdSpan = 8192;
+
+RowLayout bwd_layout(int dim, int es, bool words) {
+  const RowLayout l = row_layout(dim, es, words);
+  return l.span > kMaxRingBwdSpan ? row_layout(dim, es, false) : l;
+}
 
 // Blocks of the backward pass: what is resident at once, so that every block
 // adds up as many rows as possible before it leaves its partial sums.
-int bwd_blocks(int64_t rows, int dim, int sms) {
-  const int threads = threads_for((dim + 15) / 16);  // one block an SM past kMaxRingBwdDim
-  const int resident = std::max(1, std::min(16, 512 / threads));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, static_cast<int64_t>(sms) * resident)));
+int64_t bwd_most_blocks(int span, int sms) {
+  const int threads = threads_for((span + 15) / 16);  // one block an SM past kMaxRingBwdSpan
+  return static_cast<int64_t>(sms) * std::max(1, std::min(16, 512 / threads));
 }
 
-template <typename T, int V, int kThreads, int kBlocks>
-cudaError_t bwd_ring_mode(const NormParams& p, int blocks, cudaStream_t s) {
+template <typename T, int kLayout, int kThreads, int kBlocks>
+cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
   const int inputs = 1 + (p.y ? 1 : 0) + (p.dxn ? 1 : 0) + (p.dh ? 1 : 0);
-  const RingShape r = ring_shape(p.dim, 16, kThreads * kBlocks, slot_bytes(p, sizeof(T), V > 1, inputs));
+  const RingShape r = ring_shape(l.span, 16, kThreads * kBlocks, slot_bytes(p, sizeof(T), kLayout, inputs));
   switch (mode_of(p)) {
-    case kPreNorm: return launch_bwd_ring<T, V, kPreNorm, kThreads, kBlocks>(p, r, blocks, s);
-    case kSharedGate: return launch_bwd_ring<T, V, kSharedGate, kThreads, kBlocks>(p, r, blocks, s);
-    default: return launch_bwd_ring<T, V, kFullGate, kThreads, kBlocks>(p, r, blocks, s);
+    case kPreNorm: return launch_bwd_ring<T, kLayout, kPreNorm, kThreads, kBlocks>(p, r, blocks, s);
+    case kSharedGate: return launch_bwd_ring<T, kLayout, kSharedGate, kThreads, kBlocks>(p, r, blocks, s);
+    default: return launch_bwd_ring<T, kLayout, kFullGate, kThreads, kBlocks>(p, r, blocks, s);
   }
+}
+
+template <typename T, int kLayout>
+cudaError_t bwd_ring_width(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
+  return l.span <= 4096 ? bwd_ring_mode<T, kLayout, 256, 2>(p, l, blocks, s)
+                        : bwd_ring_mode<T, kLayout, 512, 1>(p, l, blocks, s);
 }
 
 template <typename T>
-cudaError_t launch_bwd(const NormParams& p, bool vec, int blocks, cudaStream_t s) {
-  if (p.dim > kMaxRingBwdDim) {
+cudaError_t launch_bwd(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
+  if (l.span > kMaxRingBwdSpan) {
     norm_bwd_kernel<T, kMaxNormDim / kMaxThreads><<<blocks, kMaxThreads, 0, s>>>(p);
     return cudaSuccess;
   }
-  if (p.dim <= 4096) return vec ? bwd_ring_mode<T, kV<T>, 256, 2>(p, blocks, s) : bwd_ring_mode<T, 1, 256, 2>(p, blocks, s);
-  return vec ? bwd_ring_mode<T, kV<T>, 512, 1>(p, blocks, s) : bwd_ring_mode<T, 1, 512, 1>(p, blocks, s);
+  switch (l.layout) {
+    case kWhole: return bwd_ring_width<T, kWhole>(p, l, blocks, s);
+    case kShifted: return bwd_ring_width<T, kShifted>(p, l, blocks, s);
+    default: return bwd_ring_width<T, kSingle>(p, l, blocks, s);
+  }
 }
 
 bool on(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -912,12 +1038,12 @@ int gmm_sm100_post_norm(const void* y, const void* x, const void* weight, const 
   p.w_f32 = weight_dtype == GMM_DTYPE_F32; p.gate_f32 = gate_dtype == GMM_DTYPE_F32;
   p.gate_mode = gate_mode; p.act = gate_act;
   p.scale = residual_scale; p.eps = eps; p.offset = weight_offset;
-  const bool vec = dim % (16 / static_cast<int64_t>(es)) == 0 && on(y, 16) && on(x, 16) && on(x_new, 16) && on(h, 16) &&
-                   on(weight, 16) && on(next_weight, 16) && (gate_mode == GMM_GATE_MODE_TOKEN || on(gate, 16));
+  const bool words = on(y, 16) && on(x, 16) && on(x_new, 16) && on(h, 16) && on(weight, 16) && on(next_weight, 16) &&
+                     (gate_mode == GMM_GATE_MODE_TOKEN || on(gate, 16));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = dtype == GMM_DTYPE_F32    ? launch_fwd<float>(p, vec, sms, s)
-                  : dtype == GMM_DTYPE_BF16 ? launch_fwd<__nv_bfloat16>(p, vec, sms, s)
-                                            : launch_fwd<__half>(p, vec, sms, s);
+  cudaError_t e = dtype == GMM_DTYPE_F32    ? launch_fwd<float>(p, words, sms, s)
+                  : dtype == GMM_DTYPE_BF16 ? launch_fwd<__nv_bfloat16>(p, words, sms, s)
+                                            : launch_fwd<__half>(p, words, sms, s);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? GMM_OK : set_error(GMM_ERR_CUDA, cudaGetErrorString(e));
 }
@@ -927,7 +1053,9 @@ size_t gmm_sm100_post_norm_backward_workspace_size(int64_t rows, int64_t dim) {
   if (rows <= 0 || dim <= 0 || dim > kMaxNormDim) return 0;
   int sms = 0;
   if (current_sm_count(&sms)) return 0;
-  return 2 * sizeof(float) * static_cast<size_t>(bwd_blocks(rows, static_cast<int>(dim), sms)) * dim;
+  // the largest count of any layout (a narrower span never has fewer blocks)
+  const int64_t most = std::min<int64_t>(rows, bwd_most_blocks(static_cast<int>(dim), sms));
+  return 2 * sizeof(float) * static_cast<size_t>(most) * dim;
 }
 
 int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weight, const void* gate,
@@ -974,10 +1102,11 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
   p.w_f32 = weight_dtype == GMM_DTYPE_F32; p.gate_f32 = gate_dtype == GMM_DTYPE_F32;
   p.gate_mode = gate_mode; p.act = gate_act;
   p.scale = residual_scale; p.offset = weight_offset;
-  const bool vec = dim % (16 / static_cast<int64_t>(es)) == 0 && on(y, 16) && on(x, 16) && on(dx_new, 16) && on(dh, 16) &&
-                   on(dy, 16) && on(dx, 16) && on(weight, 16) && on(next_weight, 16) &&
-                   (gate_mode == GMM_GATE_MODE_TOKEN || (on(gate, 16) && on(dgate, 16)));
-  const int blocks = bwd_blocks(rows, p.dim, sms);
+  const bool words = on(y, 16) && on(x, 16) && on(dx_new, 16) && on(dh, 16) && on(dy, 16) && on(dx, 16) &&
+                     on(weight, 16) && on(next_weight, 16) &&
+                     (gate_mode == GMM_GATE_MODE_TOKEN || (on(gate, 16) && on(dgate, 16)));
+  const RowLayout layout = bwd_layout(p.dim, static_cast<int>(es), words);
+  const int blocks = blocks_for(rows, bwd_most_blocks(layout.span, sms), layout.period);
   ReduceParams r = {};
   r.partial = p.partial;
   r.w = weight;
@@ -995,7 +1124,7 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
   const dim3 rgrid((p.dim + 31) / 32, 2);
   auto go = [&](auto t) {
     using T = decltype(t);
-    const cudaError_t e = launch_bwd<T>(p, vec, blocks, s);
+    const cudaError_t e = launch_bwd<T>(p, layout, blocks, s);
     if (e != cudaSuccess) return e;
     norm_reduce_kernel<T><<<rgrid, 1024, 0, s>>>(r);
     return cudaGetLastError();

@@ -127,13 +127,17 @@ struct RowRing {
     __syncthreads();
   }
 
-  // Where input i of the row in `slot` starts, from slot 0's start.
-  __device__ __forceinline__ uint32_t at(int slot, int i, long long row) const {
+  // Where the first word of input i of `slot` lies, from slot 0's start, and
+  // where the row in it starts.
+  __device__ __forceinline__ uint32_t word_at(int slot, int i) const {
     uint32_t off = slot * slot_bytes;
 #pragma unroll
     for (int j = 0; j < i; ++j) off += pitch(j);
-    if (!kAligned) off += static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u);
     return off;
+  }
+  __device__ __forceinline__ uint32_t at(int slot, int i, long long row) const {
+    return word_at(slot, i) +
+           (kAligned ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u));
   }
 
   // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  The

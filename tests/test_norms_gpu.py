@@ -183,6 +183,30 @@ def test_gates(gate, kind, dtype, params, D):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("gate", ["token", "full"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,D", [(21, 64), (700, 77), (1500, 250), (33, 4091), (19, 5003)])
+def test_fp32_gate_beside_16_bit_rows(T, D, dtype, gate):
+    d = inputs(T, D, dtype, dtype, gate, seed=22)
+    d["g"] = d["g"].float() * 1.01
+    want = formulas(d, "sigmoid", 0.6)
+    got = train(cuda(d), "sigmoid", 0.6)
+    assert got["dg"].dtype == torch.float32
+    for k, v in got.items():
+        check(v, want[k], k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,D", [(3000, 1), (3000, 9), (2500, 31), (1200, 255), (700, 1026), (450, 4083), (330, 8190)])
+def test_many_rows_off_the_word(T, D, dtype):
+    """Rows that start anywhere in a 16-byte word, several to a block; nothing is written outside the outputs."""
+    d = inputs(T, D, dtype, torch.float32, "channel", seed=23)
+    want = formulas(d, "tanh", 0.7)
+    got = train(cuda(d), "tanh", 0.7)
+    for k, v in got.items():
+        check(v, want[k], k)
+
+
 @pytest.mark.parametrize("use_dx,use_dh", [(True, False), (False, True)])
 @pytest.mark.parametrize("gate", ["none", "token"])
 def test_one_output_used(use_dx, use_dh, gate):
