@@ -207,12 +207,12 @@ __device__ __forceinline__ void read_unit(const void* row, int c, float* f) {
   unpack_unit<T, V>(static_cast<const RawUnit<T, V>*>(row)[c], f);
 }
 
-// The same, 0 where the unit is past the row's end (`in` false).
-template <typename T, int V>
-__device__ __forceinline__ void read_unit_or_0(const void* row, int c, bool in, float* f) {
+// The same, 0 where the unit is past the row's end (`in` false), and through `mask`.
+template <typename T, int V, typename Mask>
+__device__ __forceinline__ void read_unit_or_0(const void* row, int c, bool in, const Mask& mask, float* f) {
   RawUnit<T, V> r = {};
   if (in) r = static_cast<const RawUnit<T, V>*>(row)[c];
-  unpack_unit<T, V>(r, f);
+  unpack_unit<T, V>(mask(r), f);
 }
 
 // Unit c of a parameter or gate row that is T or fp32.
@@ -254,7 +254,7 @@ struct Span {
   __device__ __forceinline__ bool partial(int c) const { return kLayout == kShifted && (c == 0 || c == units - 1); }
   __device__ __forceinline__ int col(int c, int j) const { return c * V + j - shift; }
   __device__ __forceinline__ bool has(int c, int j) const { return col(c, j) >= 0 && col(c, j) < dim; }
-  // What a partial unit holds of other rows becomes 0.
+  // A partial unit's elements that are not the row's become 0.
   __device__ __forceinline__ void mask(int c, float* f) const {
     if (partial(c))
 #pragma unroll
@@ -270,6 +270,33 @@ struct Span {
     } else {
       write_unit<T, V>(row - shift, c, f);
     }
+  }
+};
+
+// Bits of a unit that are the row's: all ones but in a shifted row's first and
+// last unit, whose other elements are its neighbours' and read as 0.  (Masked
+// after unpacking, element by element, a forward pass of 16384 x 4001 bf16
+// took 126 us; cleared in the ring by the units' owners, 150 us.)
+template <typename T, int V, int kLayout>
+struct UnitMask {
+  __device__ __forceinline__ void set(const Span<V, kLayout>&, int) {}
+  __device__ __forceinline__ RawUnit<T, V> operator()(const RawUnit<T, V>& r) const { return r; }
+};
+template <typename T, int V>
+struct UnitMask<T, V, kShifted> {
+  uint32_t m[4];
+  __device__ __forceinline__ void set(const Span<V, kShifted>& span, int c) {
+    constexpr int kPer = 4 / static_cast<int>(sizeof(T));  // elements of a 32-bit word
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      m[w] = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (span.has(c, w * kPer + j)) m[w] |= (kPer == 1 ? 0xffffffffu : 0xffffu) << (16 * j);
+    }
+  }
+  __device__ __forceinline__ uint4 operator()(const uint4& r) const {
+    return make_uint4(r.x & m[0], r.y & m[1], r.z & m[2], r.w & m[3]);
   }
 };
 
@@ -344,7 +371,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
     return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
   };
   // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
-  const int gate_words = kLayout == kShifted && sizeof(T) == 2 && p.gate_f32 ? span.shift / 4 * 16 : 0;
+  const bool wide_gate = kLayout == kShifted && kMode == kFullGate && sizeof(T) == 2 && p.gate_f32;
+  const int gate_words = wide_gate ? span.shift / 4 * 16 : 0;
+  UnitMask<T, V, kLayout> mask[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) mask[i].set(span, threadIdx.x + i * blockDim.x);
   __syncthreads();  // barriers initialised
   const float inv_d = 1.f / static_cast<float>(D);
 
@@ -361,8 +392,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-        read_unit_or_0<T, V>(xs, c, c < units, x + i * V);
-        span.mask(c, x + i * V);
+        read_unit_or_0<T, V>(xs, c, c < units, mask[i], x + i * V);
       }
     } else {
       const auto* ys = input(1, slot, row);
@@ -371,10 +401,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-        read_unit_or_0<T, V>(ys, c, c < units, y + i * V);
-        span.mask(c, y + i * V);
+        read_unit_or_0<T, V>(ys, c, c < units, mask[i], y + i * V);
         xr[i] = RawUnit<T, V>{};
-        if (c < units) xr[i] = xs[c];
+        if (c < units) xr[i] = mask[i](xs[c]);
       }
 #pragma unroll
       for (int j = 0; j < kE; j += 2) fma2(sq, y + j, y + j, sq);
@@ -387,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
 #pragma unroll
           for (int j = 0; j < V; ++j) g[j] = 0.f;
           if (c < units) read_param<T, V>(gs, p.gate_f32, c, g);
-          span.mask(c, g);
+          if (kLayout == kShifted) span.mask(c, g);
 #pragma unroll
           for (int j = 0; j < V; ++j) y[i * V + j] *= act_of(g[j], p.act);
         }
@@ -396,10 +425,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
       if (p.rstd_y && threadIdx.x == 0) p.rstd_y[row] = ry;
       const Both c0(ry * tok);
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        unpack_unit<T, V>(xr[i], x + i * V);
-        span.mask(threadIdx.x + i * blockDim.x, x + i * V);
-      }
+      for (int i = 0; i < kUnits; ++i) unpack_unit<T, V>(xr[i], x + i * V);
 #pragma unroll
       for (int j = 0; j < kE; j += 2) {
         mul2(y + j, y + j, c0);
@@ -482,7 +508,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
     return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
   };
   // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
-  const int gate_words = kLayout == kShifted && sizeof(T) == 2 && p.gate_f32 ? span.shift / 4 * 16 : 0;
+  const bool wide_gate = kLayout == kShifted && kMode == kFullGate && sizeof(T) == 2 && p.gate_f32;
+  const int gate_words = wide_gate ? span.shift / 4 * 16 : 0;
+  UnitMask<T, V, kLayout> mask[kE / V];
+#pragma unroll
+  for (int i = 0; i < kE / V; ++i) mask[i].set(span, threadIdx.x + i * blockDim.x);
 #pragma unroll
   for (int j = 0; j < kE; ++j) acc[j] = dv[j] = 0.f;
   __syncthreads();  // barriers initialised
@@ -508,15 +538,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
       for (int k = 0; k < kU; ++k) {
         const int c = unit(g, k);
         const bool in = V > 1 || c < units;
-        read_unit_or_0<T, V>(in_x, c, in, x + k * V);
-        span.mask(c, x + k * V);
-        if constexpr (kMode != kPreNorm) {
-          read_unit_or_0<T, V>(in_y, c, in, y + k * V);
-          span.mask(c, y + k * V);
-        }
+        const auto& own = mask[g * kU + k];
+        read_unit_or_0<T, V>(in_x, c, in, own, x + k * V);
+        if constexpr (kMode != kPreNorm) read_unit_or_0<T, V>(in_y, c, in, own, y + k * V);
         if (p.dh) {
-          read_unit_or_0<T, V>(in_dh, c, in, dh + k * V);
-          span.mask(c, dh + k * V);
+          read_unit_or_0<T, V>(in_dh, c, in, own, dh + k * V);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) dh[k * V + j] = 0.f;
@@ -525,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
           if (in) read_param<T, V>(in_g, p.gate_f32, c, a + k * V);
-          span.mask(c, a + k * V);
+          if (kLayout == kShifted) span.mask(c, a + k * V);
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = act_of(a[k * V + j], p.act);
         }
@@ -545,8 +571,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_bwd_ring_kernel(const 
       for (int k = 0; k < kU; ++k) {
         const int c = unit(g, k);
         if (p.dxn) {
-          read_unit_or_0<T, V>(in_dx, c, V > 1 || c < units, d + k * V);
-          span.mask(c, d + k * V);
+          read_unit_or_0<T, V>(in_dx, c, V > 1 || c < units, mask[g * kU + k], d + k * V);
         } else {
 #pragma unroll
           for (int j = 0; j < V; ++j) d[k * V + j] = 0.f;
@@ -924,7 +949,9 @@ cudaError_t fwd_ring_mode(const NormParams& p, const RowLayout& l, int sms, cuda
 
 template <typename T, int kLayout>
 cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
-  if (l.span <= 4096) return fwd_ring_mode<T, kLayout, 8, 512, 2>(p, l, sms, s);
+  // (a shifted row of 4096 elements or fewer spans at most one warp more)
+  constexpr int kNarrow = kLayout == kShifted ? 544 : 512;
+  if (l.span <= 8 * kNarrow) return fwd_ring_mode<T, kLayout, 8, kNarrow, 2>(p, l, sms, s);
   if (l.span <= 8192) return fwd_ring_mode<T, kLayout, 8, 1024, 1>(p, l, sms, s);
   return fwd_ring_mode<T, kLayout, 16, 1024, 1>(p, l, sms, s);
 }
@@ -953,10 +980,13 @@ RowLayout bwd_layout(int dim, int es, bool words) {
 
 // Blocks of the backward pass: what is resident at once, so that every block
 // adds up as many rows as possible before it leaves its partial sums.
-int64_t bwd_most_blocks(int span, int sms) {
+int64_t bwd_most_blocks(int span, int threads_sm, int sms) {
   const int threads = threads_for((span + 15) / 16);  // one block an SM past kMaxRingBwdSpan
-  return static_cast<int64_t>(sms) * std::max(1, std::min(16, 512 / threads));
+  return static_cast<int64_t>(sms) * std::max(1, std::min(16, threads_sm / threads));
 }
+constexpr int kBwdThreadsSm = 512, kBwdThreadsSmShifted = 576;  // threads of all blocks of an SM
+
+int bwd_threads_sm(const RowLayout& l) { return l.layout == kShifted ? kBwdThreadsSmShifted : kBwdThreadsSm; }
 
 template <typename T, int kLayout, int kThreads, int kBlocks>
 cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
@@ -971,8 +1001,9 @@ cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, c
 
 template <typename T, int kLayout>
 cudaError_t bwd_ring_width(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
-  return l.span <= 4096 ? bwd_ring_mode<T, kLayout, 256, 2>(p, l, blocks, s)
-                        : bwd_ring_mode<T, kLayout, 512, 1>(p, l, blocks, s);
+  constexpr int kNarrow = (kLayout == kShifted ? kBwdThreadsSmShifted : kBwdThreadsSm) / 2;
+  return l.span <= 16 * kNarrow ? bwd_ring_mode<T, kLayout, kNarrow, 2>(p, l, blocks, s)
+                                : bwd_ring_mode<T, kLayout, 512, 1>(p, l, blocks, s);
 }
 
 template <typename T>
@@ -1054,7 +1085,7 @@ size_t gmm_sm100_post_norm_backward_workspace_size(int64_t rows, int64_t dim) {
   int sms = 0;
   if (current_sm_count(&sms)) return 0;
   // the largest count of any layout (a narrower span never has fewer blocks)
-  const int64_t most = std::min<int64_t>(rows, bwd_most_blocks(static_cast<int>(dim), sms));
+  const int64_t most = std::min<int64_t>(rows, bwd_most_blocks(static_cast<int>(dim), kBwdThreadsSmShifted, sms));
   return 2 * sizeof(float) * static_cast<size_t>(most) * dim;
 }
 
@@ -1106,7 +1137,7 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
                      on(weight, 16) && on(next_weight, 16) &&
                      (gate_mode == GMM_GATE_MODE_TOKEN || (on(gate, 16) && on(dgate, 16)));
   const RowLayout layout = bwd_layout(p.dim, static_cast<int>(es), words);
-  const int blocks = blocks_for(rows, bwd_most_blocks(layout.span, sms), layout.period);
+  const int blocks = blocks_for(rows, bwd_most_blocks(layout.span, bwd_threads_sm(layout), sms), layout.period);
   ReduceParams r = {};
   r.partial = p.partial;
   r.w = weight;
