@@ -166,8 +166,8 @@ __device__ __forceinline__ float token_gate(const NormParams& p, long long row) 
 //             parameters and sums stay in registers;
 //   kSingle   V is 1 (tensors off the 16-byte grid): neighbouring threads read
 //             neighbouring elements.
-// 16384 x 4095 bf16, channel gate: kSingle 163 us forward, 623 forward and
-// backward; 4096 columns (kWhole) 88 and 231; kShifted, see the launches.
+// 16384 x 4001 bf16, channel gate, forward, and forward and backward: kSingle
+// 160 and 600 us, kShifted 104 and 332; 4000 columns (kWhole) 88 and 231.
 enum Layout { kWhole = 0, kShifted = 1, kSingle = 2 };
 enum RingMode { kPreNorm = 0, kSharedGate = 1, kFullGate = 2 };  // no y | gate none, channel, token | gate per element
 
@@ -243,6 +243,25 @@ __device__ __forceinline__ void write_unit(T* row, int c, const float* f) {
   }
 }
 
+// Elements [col, col + V) of a row that lie in it.  A call, so that the other
+// units' path stays free of it.
+template <typename T>
+__device__ __noinline__ void write_partial_raw(T* row, int col, int dim, uint4 raw) {
+  constexpr int kN = 16 / static_cast<int>(sizeof(T));
+  const T* f = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int j = 0; j < kN; ++j)
+    if (col + j >= 0 && col + j < dim) row[col + j] = f[j];
+}
+template <typename T, int V>
+__device__ __forceinline__ void write_partial(T* row, int col, int dim, const float* f) {
+  if constexpr (V > 1) {
+    uint4 raw;
+    write_unit<T, V>(reinterpret_cast<T*>(&raw), 0, f);
+    write_partial_raw<T>(row, col, dim, raw);
+  }
+}
+
 // Which of the row's elements a unit holds.
 template <int V, int kLayout>
 struct Span {
@@ -263,13 +282,8 @@ struct Span {
   // The same unit of a row in global memory: rows of one block start at the same place in a word.
   template <typename T>
   __device__ __forceinline__ void write(T* row, int c, const float* f) const {
-    if (partial(c)) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (has(c, j)) row[col(c, j)] = from_float<T>(f[j]);
-    } else {
-      write_unit<T, V>(row - shift, c, f);
-    }
+    if (partial(c)) write_partial<T, V>(row, col(c, 0), dim, f);
+    else write_unit<T, V>(row - shift, c, f);
   }
 };
 
@@ -937,23 +951,43 @@ size_t slot_bytes(const NormParams& p, int es, int layout, int inputs) {
   return static_cast<size_t>(row_pitch(p.dim * es, whole)) * inputs + (gate ? row_pitch(gate, whole) : 0);
 }
 
-template <typename T, int kLayout, int kE, int kThreads, int kBlocks>
-cudaError_t fwd_ring_mode(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
+template <typename T, int kLayout, int kE, int kMode, int kThreads, int kBlocks>
+cudaError_t fwd_ring(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
   const RingShape r = ring_shape(l.span, kE, kThreads * kBlocks, slot_bytes(p, sizeof(T), kLayout, p.y ? 2 : 1));
-  switch (mode_of(p)) {
-    case kPreNorm: return launch_fwd_ring<T, kLayout, kE, kPreNorm, kThreads, kBlocks>(p, r, l.period, sms, s);
-    case kSharedGate: return launch_fwd_ring<T, kLayout, kE, kSharedGate, kThreads, kBlocks>(p, r, l.period, sms, s);
-    default: return launch_fwd_ring<T, kLayout, kE, kFullGate, kThreads, kBlocks>(p, r, l.period, sms, s);
+  return launch_fwd_ring<T, kLayout, kE, kMode, kThreads, kBlocks>(p, r, l.period, sms, s);
+}
+
+// Elements a thread and blocks an SM.  More elements a thread share the cost
+// of a row's sums, fewer leave registers for more warps: one B200, bf16, a
+// channel gate unless said,
+//                                8 a thread      16 a thread
+//   16384 x 4096 (whole words)      88 us           100 us
+//   16384 x 4000, gate per element  124             118
+//   16384 x 4001 (shifted)          137             104
+//   10240 x 6144                    96              92
+//   10240 x 6144, gate per element  138             111
+//   8192 x 7168                     87              75
+template <typename T, int kLayout, int kMode>
+cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
+  constexpr int kNarrow = kLayout == kShifted ? 288 : 256;  // a shifted row of 4096 spans at most one warp more
+  if (l.span <= 16 * kNarrow) {
+    if constexpr (kLayout != kShifted && kMode != kFullGate)
+      return fwd_ring<T, kLayout, 8, kMode, 512, 2>(p, l, sms, s);
+    else
+      return fwd_ring<T, kLayout, 16, kMode, kNarrow, 3 * 256 / kNarrow>(p, l, sms, s);
   }
+  if (l.span <= 6144) return fwd_ring<T, kLayout, 16, kMode, 384, 2>(p, l, sms, s);
+  if (l.span <= 8192) return fwd_ring<T, kLayout, 16, kMode, 512, 1>(p, l, sms, s);
+  return fwd_ring<T, kLayout, 16, kMode, 1024, 1>(p, l, sms, s);
 }
 
 template <typename T, int kLayout>
-cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
-  // (a shifted row of 4096 elements or fewer spans at most one warp more)
-  constexpr int kNarrow = kLayout == kShifted ? 544 : 512;
-  if (l.span <= 8 * kNarrow) return fwd_ring_mode<T, kLayout, 8, kNarrow, 2>(p, l, sms, s);
-  if (l.span <= 8192) return fwd_ring_mode<T, kLayout, 8, 1024, 1>(p, l, sms, s);
-  return fwd_ring_mode<T, kLayout, 16, 1024, 1>(p, l, sms, s);
+cudaError_t fwd_ring_mode(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
+  switch (mode_of(p)) {
+    case kPreNorm: return fwd_ring_width<T, kLayout, kPreNorm>(p, l, sms, s);
+    case kSharedGate: return fwd_ring_width<T, kLayout, kSharedGate>(p, l, sms, s);
+    default: return fwd_ring_width<T, kLayout, kFullGate>(p, l, sms, s);
+  }
 }
 
 constexpr int kMaxRingFwdSpan = 16384;
@@ -963,9 +997,9 @@ cudaError_t launch_fwd(const NormParams& p, bool words, int sms, cudaStream_t s)
   RowLayout l = row_layout(p.dim, sizeof(T), words);
   if (l.span > kMaxRingFwdSpan) l = row_layout(p.dim, sizeof(T), false);
   switch (l.layout) {
-    case kWhole: return fwd_ring_width<T, kWhole>(p, l, sms, s);
-    case kShifted: return fwd_ring_width<T, kShifted>(p, l, sms, s);
-    default: return fwd_ring_width<T, kSingle>(p, l, sms, s);
+    case kWhole: return fwd_ring_mode<T, kWhole>(p, l, sms, s);
+    case kShifted: return fwd_ring_mode<T, kShifted>(p, l, sms, s);
+    default: return fwd_ring_mode<T, kSingle>(p, l, sms, s);
   }
 }
 
@@ -978,15 +1012,14 @@ RowLayout bwd_layout(int dim, int es, bool words) {
   return l.span > kMaxRingBwdSpan ? row_layout(dim, es, false) : l;
 }
 
+constexpr int kBwdThreadsSm = 512;  // threads of all blocks of an SM (128 registers each)
+
 // Blocks of the backward pass: what is resident at once, so that every block
 // adds up as many rows as possible before it leaves its partial sums.
-int64_t bwd_most_blocks(int span, int threads_sm, int sms) {
+int64_t bwd_most_blocks(int span, int sms) {
   const int threads = threads_for((span + 15) / 16);  // one block an SM past kMaxRingBwdSpan
-  return static_cast<int64_t>(sms) * std::max(1, std::min(16, threads_sm / threads));
+  return static_cast<int64_t>(sms) * std::max(1, std::min(16, kBwdThreadsSm / threads));
 }
-constexpr int kBwdThreadsSm = 512, kBwdThreadsSmShifted = 576;  // threads of all blocks of an SM
-
-int bwd_threads_sm(const RowLayout& l) { return l.layout == kShifted ? kBwdThreadsSmShifted : kBwdThreadsSm; }
 
 template <typename T, int kLayout, int kThreads, int kBlocks>
 cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
@@ -1001,9 +1034,8 @@ cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, c
 
 template <typename T, int kLayout>
 cudaError_t bwd_ring_width(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
-  constexpr int kNarrow = (kLayout == kShifted ? kBwdThreadsSmShifted : kBwdThreadsSm) / 2;
-  return l.span <= 16 * kNarrow ? bwd_ring_mode<T, kLayout, kNarrow, 2>(p, l, blocks, s)
-                                : bwd_ring_mode<T, kLayout, 512, 1>(p, l, blocks, s);
+  return l.span <= 4096 ? bwd_ring_mode<T, kLayout, 256, 2>(p, l, blocks, s)
+                        : bwd_ring_mode<T, kLayout, 512, 1>(p, l, blocks, s);
 }
 
 template <typename T>
@@ -1085,7 +1117,7 @@ size_t gmm_sm100_post_norm_backward_workspace_size(int64_t rows, int64_t dim) {
   int sms = 0;
   if (current_sm_count(&sms)) return 0;
   // the largest count of any layout (a narrower span never has fewer blocks)
-  const int64_t most = std::min<int64_t>(rows, bwd_most_blocks(static_cast<int>(dim), kBwdThreadsSmShifted, sms));
+  const int64_t most = std::min<int64_t>(rows, bwd_most_blocks(static_cast<int>(dim), sms));
   return 2 * sizeof(float) * static_cast<size_t>(most) * dim;
 }
 
@@ -1137,7 +1169,7 @@ int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weigh
                      on(weight, 16) && on(next_weight, 16) &&
                      (gate_mode == GMM_GATE_MODE_TOKEN || (on(gate, 16) && on(dgate, 16)));
   const RowLayout layout = bwd_layout(p.dim, static_cast<int>(es), words);
-  const int blocks = blocks_for(rows, bwd_most_blocks(layout.span, bwd_threads_sm(layout), sms), layout.period);
+  const int blocks = blocks_for(rows, bwd_most_blocks(layout.span, sms), layout.period);
   ReduceParams r = {};
   r.partial = p.partial;
   r.w = weight;

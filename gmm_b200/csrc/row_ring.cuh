@@ -52,6 +52,7 @@ struct RowRing {
   uint32_t slot_bytes;
   uint32_t bars;            // shared address of the slots' barriers
   int slots;
+  int edge_rows;            // rows at either end of a tensor within 15 bytes of it
   bool dead;                // a wait ran out: no more waiting or loading, the error word says so
 
   __device__ __forceinline__ uint32_t pitch(int i) const { return bytes[i] ? row_pitch(bytes[i], kAligned) : 0; }
@@ -87,12 +88,7 @@ struct RowRing {
   // Whether the words of `row` may reach beyond an input's first or last byte
   // (they reach at most 15 bytes past the row on either side).
   __device__ __forceinline__ bool edge(long long row) const {
-    if (kAligned) return false;
-    long long least = INT64_MAX;
-#pragma unroll
-    for (int i = 0; i < kInputs; ++i)
-      if (bytes[i]) least = min(least, static_cast<long long>(bytes[i]));
-    return row * least < 15 || (rows - 1 - row) * least < 15;
+    return !kAligned && (row < edge_rows || row >= rows - edge_rows);
   }
 
   // All threads: wait for the row in `slot`.
@@ -148,8 +144,13 @@ struct RowRing {
     rows = num_rows;
     dead = false;
     slot_bytes = 0;
+    uint32_t least = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < kInputs; ++i) slot_bytes += pitch(i);
+    for (int i = 0; i < kInputs; ++i) {
+      slot_bytes += pitch(i);
+      if (bytes[i]) least = min(least, bytes[i]);
+    }
+    edge_rows = (15 + least - 1) / least;
     bars = smem_u32(mem) + slots * slot_bytes;
     if (threadIdx.x == 0) {
       for (int s = 0; s < slots; ++s) mbar_init(bars + 8 * s, 1);
