@@ -942,6 +942,7 @@ __global__ void __launch_bounds__(32) ep_barrier_kernel(const __grid_constant__ 
 #include "gmm_pair_kernel.cuh"
 #include "gmm_vark_kernel.cuh"
 #include "gmm_swap_kernel.cuh"
+#include "gmm_stream_kernel.cuh"
 
 }  // namespace gmm_sm100
 
@@ -1195,6 +1196,44 @@ int launch_swap(const GmmParams& prm, int grid, cudaStream_t stream, DeviceInfo*
                      "gmm swap kernel launch");
 }
 
+// Launch the streaming kernel (8-bit operands, few rows an expert).  At most
+// `tiles` (row block, 256-column) tiles: a block for each of their tasks, up to
+// what is resident at once.
+template <int kTableInts>
+int launch_stream_table(StreamParams<kTableInts>& sp, const GmmParams& prm, const void* A, const void* B, int64_t K,
+                        int64_t N, int dtype, int act, int tiles, DeviceInfo* di, cudaStream_t stream) {
+  sp.a = static_cast<const int8_t*>(A);
+  sp.b = static_cast<const int8_t*>(B);
+  sp.k = K;
+  sp.b_cols = N;
+  sp.n_tiles = (prm.dim_out + kStreamCols - 1) / kStreamCols;
+  const int64_t tasks = static_cast<int64_t>(tiles) * (256 / kStreamCols);
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, kStreamBlocksSm * di->sm_count)));
+  auto go = [&](auto kernel) {
+    kernel<<<grid, kStreamWarps * 32, 0, stream>>>(sp);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? GMM_OK : cuda_fail(e, "gmm stream kernel launch");
+  };
+  if (act) return dtype == GMM_DTYPE_BF16 ? go(gmm_stream_kernel<2, __nv_bfloat16, kTableInts>)
+                                          : go(gmm_stream_kernel<2, __half, kTableInts>);
+  if (dtype == GMM_DTYPE_BF16) return go(gmm_stream_kernel<1, __nv_bfloat16, kTableInts>);
+  if (dtype == GMM_DTYPE_F16) return go(gmm_stream_kernel<1, __half, kTableInts>);
+  return go(gmm_stream_kernel<1, float, kTableInts>);
+}
+
+int launch_stream(const GmmParams& prm, const void* A, const void* B, int64_t K, int64_t N, int dtype, int act,
+                  int tiles, DeviceInfo* di, cudaStream_t stream) {
+  if (int rc = check_table(prm)) return rc;
+  if (prm.inline_ints <= kSmallTableInts) {
+    StreamParams<kSmallTableInts> sp;
+    small_params(prm, sp);
+    return launch_stream_table(sp, prm, A, B, K, N, dtype, act, tiles, di, stream);
+  }
+  StreamParams<kInlineTableInts> sp;
+  static_cast<GmmParams&>(sp) = prm;
+  return launch_stream_table(sp, prm, A, B, K, N, dtype, act, tiles, di, stream);
+}
+
 // Tile kind of a problem.  fp32: 128-row tiles.  16-bit: CTA-pair 256-row
 // tiles when the non-empty experts average at least 384 rows; swap-AB tiles
 // when no expert has more than 64 rows (decode-shaped routing, where a
@@ -1204,7 +1243,9 @@ int launch_swap(const GmmParams& prm, int grid, cudaStream_t stream, DeviceInfo*
 // GMM_SM100_TILE=128 / 256 / swap, read once) forces one of them (swap falls
 // back to 128 for the SwiGLU and expert-parallel epilogues, which it does not
 // have).
-enum TileKind { kTile128 = 0, kTilePair = 1, kTileSwap = 2 };
+// 8-bit operands: CTA pairs and 128-row tiles by the same rule, and the
+// streaming kernel when no expert has more than 16 rows (or "swap" is forced).
+enum TileKind { kTile128 = 0, kTilePair = 1, kTileSwap = 2, kTileStream = 3 };
 
 std::atomic<int> g_tile_force{-1};  // a gmm_tile_kind; -1 = not initialised yet
 std::once_flag g_tile_force_once;
@@ -1228,13 +1269,14 @@ TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int dtype, in
   const int force = tile_force();
   if (force == GMM_TILE_128) return kTile128;
   if (force == GMM_TILE_PAIR) return kTilePair;
-  if (force == GMM_TILE_SWAP) return swap_ok ? kTileSwap : kTile128;
+  if (force == GMM_TILE_SWAP) return i8 ? kTileStream : (swap_ok ? kTileSwap : kTile128);
   int64_t groups = 0, max_m = 0;
   for (int64_t e = 0; e < E; ++e) {
     groups += bs[e] > 0;
     max_m = std::max(max_m, bs[e]);
   }
   if (groups > 0 && T >= 384 * groups) return kTilePair;
+  if (i8 && max_m <= kStreamRows) return kTileStream;
   return (swap_ok && max_m <= 64) ? kTileSwap : kTile128;
 }
 
@@ -1283,6 +1325,8 @@ int setup_and_launch(GmmParams& prm, const void* A, const void* B, int64_t T, in
                      cudaStream_t stream, bool swap = false, bool i8 = false) {
   int rc = GMM_OK;
   const cuuint64_t uT = T, uK = K, uN = N, uE = E;
+  if (i8 && tile_rows == kStreamRows)
+    return launch_stream(prm, A, B, K, N, dtype, act, grid_tiles, di, stream);
   if (i8) {  // A and B[e] ([N, K]) are K-major: boxes of 128 bytes of K, rows as for the 16-bit kinds
     const CUtensorMapDataType tt = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const cuuint64_t adims[2] = {uK, uT}, astr[1] = {uK};
@@ -1381,7 +1425,7 @@ int plan_impl(const int64_t* batch_sizes, int64_t num_experts, int64_t num_token
   int rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl, 128, i8);
   if (rc != GMM_OK) return rc;
   po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dtype, act, remote, i8);
-  po.tile_rows = po.kind == kTilePair ? 256 : 128;
+  po.tile_rows = po.kind == kTilePair ? 256 : (po.kind == kTileStream ? kStreamRows : 128);
   if (po.tile_rows != 128 && (rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl,
                                              po.tile_rows, i8)) != GMM_OK)
     return rc;
@@ -1582,12 +1626,14 @@ int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_de
   bool swap = false;
   if (dtype != GMM_DTYPE_F32 || i8) {
     const int force = tile_force();
+    bool few = force == GMM_TILE_SWAP;
     if (force == GMM_TILE_PAIR) tile_rows = 256;
-    else if (force == GMM_TILE_SWAP) swap = !swiglu && !i8;
-    else if (force != GMM_TILE_128) {
+    else if (force == GMM_TILE_AUTO) {
       if (T >= 384 * E) tile_rows = 256;
-      else swap = !swiglu && !i8 && T <= 16 * E;
+      else few = T <= 16 * E;
     }
+    if (few && i8) tile_rows = kStreamRows;
+    else if (few) swap = !swiglu;
   }
   const int64_t BN = dtype == GMM_DTYPE_F32 && !i8 ? 128 : 256;
   const int64_t BK = i8 ? 128 : (dtype == GMM_DTYPE_F32 ? 32 : 64);

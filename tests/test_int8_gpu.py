@@ -38,7 +38,7 @@ def _device():
     assert capi.device_error(clear=True) == 0
 
 
-@pytest.fixture(params=["auto", "128", "256"])
+@pytest.fixture(params=["auto", "128", "256", "swap"])
 def tile(request):
     with forced_tile(request.param):
         yield request.param
@@ -85,6 +85,8 @@ RAGGED = [
     ([0, 0, 257, 0], 1040, 520),
     ([400, 513, 385], 272, 520),                   # CTA-pair tiles with half-tile tails
     ([1] * 130 + [0] * 20, 80, 40),                # more groups than the small inline table
+    ([16, 1, 0, 9, 15, 8], 2064, 48),              # decode: at most 16 rows an expert, the contraction split over warps
+    ([2] * 100, 336, 328),                         # decode: more tasks than warps
 ]
 
 
@@ -102,7 +104,8 @@ def test_gmm_int8(bs, dim, dim_out, out, tile):
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("bs,dim,dim_out", [([1], 16, 16), ([127, 0, 130, 1], 208, 272), ([500, 390], 144, 528)])
+@pytest.mark.parametrize("bs,dim,dim_out", [([1], 16, 16), ([127, 0, 130, 1], 208, 272), ([500, 390], 144, 528),
+                                            ([1, 16, 0, 9], 2064, 96), ([5] * 90, 160, 336)])
 def test_gmm_int8_swiglu(bs, dim, dim_out, out, tile):
     from gmm_b200.int8 import gmm_int8, gmm_int8_dev
     p = problem(bs, dim, dim_out, seed=1)
