@@ -994,7 +994,8 @@ struct DeviceInfo {
   // Bit per kernel variant whose shared-memory attribute is set: 0 fp32;
   // 1-4 128-row bf16/fp16 x NT/NN; 5-8 CTA pair; 9-10 variable-K bf16/fp16;
   // 11-14 swap-AB bf16/fp16 x NT/NN; 32-34 128-row, 35-37 CTA pair with 8-bit
-  // operands and bf16/fp16/fp32 output.  Small-table instantiations: bit + 16.
+  // operands and bf16/fp16/fp32 output, 38-42 streaming kernel.  The other
+  // instantiation of the parameter block (small, or full for streaming): bit + 16.
   std::atomic<unsigned long long> smem_attr_set{0};
   int pair_clusters[64] = {};               // resident CTA pairs per pair-kernel variant
 };
@@ -1209,16 +1210,19 @@ int launch_stream_table(StreamParams<kTableInts>& sp, const GmmParams& prm, cons
   sp.n_tiles = (prm.dim_out + kStreamCols - 1) / kStreamCols;
   const int64_t tasks = static_cast<int64_t>(tiles) * (256 / kStreamCols);
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tasks, kStreamBlocksSm * di->sm_count)));
-  auto go = [&](auto kernel) {
-    kernel<<<grid, kStreamWarps * 32, 0, stream>>>(sp);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? GMM_OK : cuda_fail(e, "gmm stream kernel launch");
+  // bits 38-42 of smem_attr_set for the small table, 16 more for the full one
+  constexpr int kBit = kTableInts == kSmallTableInts ? 38 : 54;
+  using Kernel = void (*)(StreamParams<kTableInts>);
+  auto go = [&](Kernel kernel, int smem, int bit) {
+    return launch_with(kernel, sp, grid, smem, stream, di, kBit + bit, "gmm stream kernel launch");
   };
-  if (act) return dtype == GMM_DTYPE_BF16 ? go(gmm_stream_kernel<2, __nv_bfloat16, kTableInts>)
-                                          : go(gmm_stream_kernel<2, __half, kTableInts>);
-  if (dtype == GMM_DTYPE_BF16) return go(gmm_stream_kernel<1, __nv_bfloat16, kTableInts>);
-  if (dtype == GMM_DTYPE_F16) return go(gmm_stream_kernel<1, __half, kTableInts>);
-  return go(gmm_stream_kernel<1, float, kTableInts>);
+  static_assert(kStreamWarps * 32 == kThreads, "launch_with");
+  constexpr int kOne = StreamCfg<1>::kSmemBytes, kTwo = StreamCfg<2>::kSmemBytes;
+  if (act) return dtype == GMM_DTYPE_BF16 ? go(gmm_stream_kernel<2, __nv_bfloat16, kTableInts>, kTwo, 0)
+                                          : go(gmm_stream_kernel<2, __half, kTableInts>, kTwo, 1);
+  if (dtype == GMM_DTYPE_BF16) return go(gmm_stream_kernel<1, __nv_bfloat16, kTableInts>, kOne, 2);
+  if (dtype == GMM_DTYPE_F16) return go(gmm_stream_kernel<1, __half, kTableInts>, kOne, 3);
+  return go(gmm_stream_kernel<1, float, kTableInts>, kOne, 4);
 }
 
 int launch_stream(const GmmParams& prm, const void* A, const void* B, int64_t K, int64_t N, int dtype, int act,
@@ -1263,20 +1267,24 @@ int tile_force() {
   return g_tile_force.load(std::memory_order_relaxed);
 }
 
-TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int dtype, int act, bool remote, bool i8) {
+// Whether the streaming kernel can count the tasks of `blocks` row blocks and N columns of B.
+bool stream_fits(int64_t blocks, int64_t N) { return blocks <= INT32_MAX / (N / kStreamCols + 1); }
+
+TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t N, int dtype, int act, bool remote, bool i8) {
   if (dtype == GMM_DTYPE_F32 && !i8) return kTile128;
   const bool swap_ok = !act && !remote && !i8;
   const int force = tile_force();
   if (force == GMM_TILE_128) return kTile128;
   if (force == GMM_TILE_PAIR) return kTilePair;
-  if (force == GMM_TILE_SWAP) return i8 ? kTileStream : (swap_ok ? kTileSwap : kTile128);
+  if (force == GMM_TILE_SWAP && i8) return stream_fits(E + T / kStreamRows, N) ? kTileStream : kTile128;
+  if (force == GMM_TILE_SWAP) return swap_ok ? kTileSwap : kTile128;
   int64_t groups = 0, max_m = 0;
   for (int64_t e = 0; e < E; ++e) {
     groups += bs[e] > 0;
     max_m = std::max(max_m, bs[e]);
   }
   if (groups > 0 && T >= 384 * groups) return kTilePair;
-  if (i8 && max_m <= kStreamRows) return kTileStream;
+  if (i8 && max_m <= kStreamRows && stream_fits(groups, N)) return kTileStream;
   return (swap_ok && max_m <= 64) ? kTileSwap : kTile128;
 }
 
@@ -1424,7 +1432,7 @@ int plan_impl(const int64_t* batch_sizes, int64_t num_experts, int64_t num_token
   NvtxRange range("gmm_sm100 plan");
   int rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl, 128, i8);
   if (rc != GMM_OK) return rc;
-  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dtype, act, remote, i8);
+  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dim_out, dtype, act, remote, i8);
   po.tile_rows = po.kind == kTilePair ? 256 : (po.kind == kTileStream ? kStreamRows : 128);
   if (po.tile_rows != 128 && (rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl,
                                              po.tile_rows, i8)) != GMM_OK)
@@ -1632,7 +1640,7 @@ int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_de
       if (T >= 384 * E) tile_rows = 256;
       else few = T <= 16 * E;
     }
-    if (few && i8) tile_rows = kStreamRows;
+    if (few && i8) tile_rows = stream_fits(E + T / kStreamRows, N) ? kStreamRows : 128;
     else if (few) swap = !swiglu;
   }
   const int64_t BN = dtype == GMM_DTYPE_F32 && !i8 ? 128 : 256;
