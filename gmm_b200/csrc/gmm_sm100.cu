@@ -1248,7 +1248,8 @@ int launch_stream(const GmmParams& prm, const void* A, const void* B, int64_t K,
 // back to 128 for the SwiGLU and expert-parallel epilogues, which it does not
 // have).
 // 8-bit operands: CTA pairs and 128-row tiles by the same rule, and the
-// streaming kernel when no expert has more than 16 rows (or "swap" is forced).
+// streaming kernel when no expert has more than 16 rows and the weights are
+// few (stream_pays), or when "swap" is forced.
 enum TileKind { kTile128 = 0, kTilePair = 1, kTileSwap = 2, kTileStream = 3 };
 
 std::atomic<int> g_tile_force{-1};  // a gmm_tile_kind; -1 = not initialised yet
@@ -1270,7 +1271,20 @@ int tile_force() {
 // Whether the streaming kernel can count the tasks of `blocks` row blocks and N columns of B.
 bool stream_fits(int64_t blocks, int64_t N) { return blocks <= INT32_MAX / (N / kStreamCols + 1); }
 
-TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t N, int dtype, int act, bool remote, bool i8) {
+// Whether few-row experts with `live` weight matrices of N x K bytes go to the
+// streaming kernel: it starts sooner and spreads small problems over every SM,
+// the 128-row tiles keep more of a long stream in flight.  One B200, bf16 out,
+// us, 8 rows an expert, streaming against 128-row tiles:
+//    2 x 768 x 2048 (3 MB)       5.9   9.4     64 x 768 x 2048 (101 MB)  24.9  25.5
+//    8 x 2048 x 1536 (25 MB)    10.5  17.4    128 x 768 x 2048 (201 MB)  42.2  40.2
+//    4 x 7168 x 4096 (117 MB)   26.5  32.2      8 x 7168 x 4096 (235 MB) 47.5  44.2
+//   32 x 768 x 2048 (50 MB)     14.8  17.0     64 x 2048 x 1536 (201 MB) 44.4  42.5
+constexpr double kStreamBytes = 1e8;
+bool stream_pays(int64_t live, int64_t K, int64_t N) {
+  return static_cast<double>(live) * static_cast<double>(K) * static_cast<double>(N) <= kStreamBytes;
+}
+
+TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t K, int64_t N, int dtype, int act, bool remote, bool i8) {
   if (dtype == GMM_DTYPE_F32 && !i8) return kTile128;
   const bool swap_ok = !act && !remote && !i8;
   const int force = tile_force();
@@ -1284,7 +1298,7 @@ TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t N, in
     max_m = std::max(max_m, bs[e]);
   }
   if (groups > 0 && T >= 384 * groups) return kTilePair;
-  if (i8 && max_m <= kStreamRows && stream_fits(groups, N)) return kTileStream;
+  if (i8 && max_m <= kStreamRows && stream_pays(groups, K, N) && stream_fits(groups, N)) return kTileStream;
   return (swap_ok && max_m <= 64) ? kTileSwap : kTile128;
 }
 
@@ -1432,7 +1446,7 @@ int plan_impl(const int64_t* batch_sizes, int64_t num_experts, int64_t num_token
   NvtxRange range("gmm_sm100 plan");
   int rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl, 128, i8);
   if (rc != GMM_OK) return rc;
-  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dim_out, dtype, act, remote, i8);
+  po.kind = choose_tile_kind(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, act, remote, i8);
   po.tile_rows = po.kind == kTilePair ? 256 : (po.kind == kTileStream ? kStreamRows : 128);
   if (po.tile_rows != 128 && (rc = make_plan(batch_sizes, num_experts, num_tokens, dim, dim_out, dtype, po.pl,
                                              po.tile_rows, i8)) != GMM_OK)
@@ -1638,7 +1652,7 @@ int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_de
     if (force == GMM_TILE_PAIR) tile_rows = 256;
     else if (force == GMM_TILE_AUTO) {
       if (T >= 384 * E) tile_rows = 256;
-      else few = T <= 16 * E;
+      else few = T <= 16 * E && (!i8 || stream_pays(std::min(E, T), K, N));
     }
     if (few && i8) tile_rows = stream_fits(E + T / kStreamRows, N) ? kStreamRows : 128;
     else if (few) swap = !swiglu;

@@ -24,6 +24,26 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// Two fp32 operations in one instruction, each rounded like its own.
+__device__ __forceinline__ void fma2(float* d, const float* a, const float* b, const float* c) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d[0]), "=f"(d[1])
+      : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+}
+__device__ __forceinline__ void mul2(float* d, const float* a, const float* b) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d[0]), "=f"(d[1])
+      : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+// A number for both halves.
+struct Both {
+  float v[2];
+  __device__ __forceinline__ explicit Both(float f) : v{f, f} {}
+  __device__ __forceinline__ operator const float*() const { return v; }
+};
+
 // Eight elements as they lie in memory.
 template <typename T>
 struct Raw8 {
