@@ -13,6 +13,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -26,11 +27,12 @@ LIB = os.path.join(PKG, "libgmm_sm100.so")
 TORCH_OP = os.path.join(PKG, "_C.so")
 
 KERNEL_SOURCES = [os.path.join(CSRC, f) for f in ("gmm_sm100.cu", "moe_sm100.cu", "quant_sm100.cu",
-                                                       "norm_sm100.cu")]
+                                                       "norm_fwd_sm100.cu", "norm_bwd_sm100.cu")]
 KERNEL_HEADERS = [os.path.join(CSRC, "gmm_pair_kernel.cuh"),
                   os.path.join(CSRC, "gmm_vark_kernel.cuh"),
                   os.path.join(CSRC, "gmm_swap_kernel.cuh"),
                   os.path.join(CSRC, "row_vec.cuh"), os.path.join(CSRC, "row_ring.cuh"),
+                  os.path.join(CSRC, "norm_sm100.cuh"), os.path.join(CSRC, "gmm_stream_kernel.cuh"),
                   os.path.join(CSRC, "sm100_ptx.cuh"),
                   os.path.join(CSRC, "status.h"),
                   os.path.join(INCLUDE, "gmm_sm100.h")]
@@ -50,10 +52,21 @@ def _run(cmd, verbose):
 
 
 def build_kernels(force=False, verbose=True, extra=()):
-    if force or _stale(LIB, KERNEL_SOURCES + KERNEL_HEADERS):
-        # the sources compile side by side (nvcc --threads)
-        _run([NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "--threads", str(len(KERNEL_SOURCES)),
-              "-Xcompiler", "-fPIC", "-shared", "-I", INCLUDE, *extra, "-o", LIB, *KERNEL_SOURCES], verbose)
+    if not (force or _stale(LIB, KERNEL_SOURCES + KERNEL_HEADERS)):
+        return LIB
+    flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", INCLUDE, *extra]
+    with tempfile.TemporaryDirectory() as tmp:  # one object a source, side by side
+        objects = [os.path.join(tmp, os.path.basename(s) + ".o") for s in KERNEL_SOURCES]
+        jobs = []
+        for src, obj in zip(KERNEL_SOURCES, objects):
+            cmd = [NVCC, *flags, "-c", "-o", obj, src]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            jobs.append((cmd, subprocess.Popen(cmd)))
+        failed = [cmd for cmd, job in jobs if job.wait() != 0]
+        if failed:
+            raise subprocess.CalledProcessError(1, failed[0])
+        _run([NVCC, *ARCH, "-shared", "-o", LIB, *objects], verbose)
     return LIB
 
 

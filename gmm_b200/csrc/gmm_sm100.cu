@@ -2050,10 +2050,12 @@ int gmm_sm100_device_error(int* status_out, int clear) {
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpyToSymbol(g_device_error)");
   }
-  int norm = 0, quant = 0;
-  if (int rc = norm_device_error(&norm, clear != 0)) return rc;
-  if (int rc = quant_device_error(&quant, clear != 0)) return rc;
-  if (status_out) *status_out = v ? v : (norm ? norm : quant);
+  for (auto read : {norm_fwd_device_error, norm_bwd_device_error, quant_device_error}) {
+    int w = 0;
+    if (int rc = read(&w, clear != 0)) return rc;
+    if (v == 0) v = w;
+  }
+  if (status_out) *status_out = v;
   return GMM_OK;
 }
 

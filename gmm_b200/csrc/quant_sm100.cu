@@ -135,8 +135,7 @@ __global__ void __launch_bounds__(512, 2) quantize_ring_kernel(const QuantParams
   __shared__ uint32_t warp_max[2][32];
   uint8_t* staged = smem;  // 2 rows of codes
   RowRing<1, kVec> ring;
-  ring.src[0] = static_cast<const char*>(p.x);
-  ring.bytes[0] = p.dim * sizeof(T);
+  ring.input(0, p.x, sizeof(T), p.dim, p.dim);
   ring.start(smem + 2 * p.dim_padded, slots, p.rows);
   __syncthreads();
   const int lane = threadIdx.x & 31;

@@ -46,7 +46,8 @@ __host__ __device__ constexpr uint32_t row_pitch(uint32_t row_bytes, bool aligne
 template <int kInputs, bool kAligned>
 struct RowRing {
   const char* src[kInputs];
-  uint32_t bytes[kInputs];  // of a row; 0: input not there
+  uint32_t bytes[kInputs];  // of a row (or of the part of it that is wanted); 0: input not there
+  long long pitch_bytes[kInputs];  // from a row to the next
   long long rows;
   uint8_t* smem;            // slot 0
   uint32_t slot_bytes;
@@ -65,7 +66,7 @@ struct RowRing {
     uint32_t len[kInputs], to[kInputs], total = 0, at = smem_u32(smem) + slot * slot_bytes;
 #pragma unroll
     for (int i = 0; i < kInputs; ++i) {
-      from[i] = src[i] + row * bytes[i];
+      from[i] = src[i] + row * pitch_bytes[i];
       len[i] = bytes[i];
       to[i] = at;
       if (!kAligned && bytes[i]) {
@@ -111,7 +112,7 @@ struct RowRing {
     uint8_t* base = smem + slot * slot_bytes;
 #pragma unroll
     for (int i = 0; i < kInputs; ++i) {
-      const char* from = src[i] + row * bytes[i];
+      const char* from = src[i] + row * pitch_bytes[i];
       const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 15u);
       const uint32_t lo = (off + 15u) & ~15u, hi = (off + bytes[i]) & ~15u, end = off + bytes[i];
       for (uint32_t k = off + 2 * threadIdx.x; k < end; k += 2 * blockDim.x)
@@ -133,7 +134,14 @@ struct RowRing {
   }
   __device__ __forceinline__ uint32_t at(int slot, int i, long long row) const {
     return word_at(slot, i) +
-           (kAligned ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * bytes[i]) & 15u));
+           (kAligned ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[i] + row * pitch_bytes[i]) & 15u));
+  }
+
+  // Input i: `n` elements of every row, `pitch` elements apart.
+  __device__ __forceinline__ void input(int i, const void* first, int elem, int n, int pitch) {
+    src[i] = static_cast<const char*>(first);
+    bytes[i] = n * elem;
+    pitch_bytes[i] = static_cast<long long>(pitch) * elem;
   }
 
   // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  The

@@ -11,7 +11,8 @@ int set_error(int code, const char* msg) noexcept;
 int current_sm_count(int* sms);
 
 // The norm and quantiser kernels' parts of gmm_sm100_device_error.
-int norm_device_error(int* status, bool clear);
+int norm_fwd_device_error(int* status, bool clear);
+int norm_bwd_device_error(int* status, bool clear);
 int quant_device_error(int* status, bool clear);
 
 }  // namespace gmm_sm100

@@ -207,6 +207,18 @@ def test_many_rows_off_the_word(T, D, dtype):
         check(v, want[k], k)
 
 
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("dtype,params", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("T,D", [(1, 8193), (200, 8200), (170, 16383), (160, 16384), (9, 12288)])
+def test_wide_rows(T, D, dtype, params, gate):
+    """Backward in column windows: each row's sums are put together from the windows'."""
+    d = inputs(T, D, dtype, params, gate, seed=24)
+    want = formulas(d, "sigmoid", 0.6)
+    got = train(cuda(d), "sigmoid", 0.6)
+    for k, v in got.items():
+        check(v, want[k], k)
+
+
 @pytest.mark.parametrize("use_dx,use_dh", [(True, False), (False, True)])
 @pytest.mark.parametrize("gate", ["none", "token"])
 def test_one_output_used(use_dx, use_dh, gate):
