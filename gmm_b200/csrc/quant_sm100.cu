@@ -259,7 +259,7 @@ extern "C" int gmm_sm100_quantize_rows(const void* x, int dtype, int64_t num_row
                                        void* stream) {
   using namespace gmm_sm100;
   if (num_rows < 0 || dim < 0 || out_rows < 0) return set_error(GMM_ERR_INVALID_ARGUMENT, "negative size");
-  if (k < 1 || k > 32 || (!dst_pos && k != 1))
+  if (k < 1 || k > 32 || (!dst_pos && k != 1 && num_rows > 0))
     return set_error(GMM_ERR_INVALID_ARGUMENT, "need 1 <= k <= 32, and k = 1 without dst_pos");
   if (dtype != GMM_DTYPE_F32 && dtype != GMM_DTYPE_BF16 && dtype != GMM_DTYPE_F16)
     return set_error(GMM_ERR_DTYPE, "rows must be fp32, bf16 or fp16");

@@ -171,7 +171,7 @@ def moe_block(x: torch.Tensor, h: torch.Tensor, w_router: torch.Tensor, w_gate_u
     expert weights are tensors (``moe_forward``) or ``quantize_experts`` pairs
     (``moe_forward_int8``).  Returns what :func:`gmm_b200.norms.post_norm` does:
     the new residual stream, and with ``next_weight`` the next block's ``h``."""
-    layer = moe_forward_int8 if isinstance(w_gate_up, tuple) else moe_forward
+    layer = moe_forward if isinstance(w_gate_up, torch.Tensor) else moe_forward_int8
     y = layer(h, torch.matmul(h, w_router), w_gate_up, w_down, k, renormalize=renormalize)
     return post_norm(y, x, post_weight, gate=gate, gate_act=gate_act, residual_scale=residual_scale,
                      next_weight=next_weight, eps=eps, weight_offset=weight_offset)

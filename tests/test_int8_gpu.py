@@ -423,6 +423,54 @@ def test_moe_forward_int8_is_its_parts_and_ffn_agrees():
     assert torch.equal(moe_ffn_int8(xp, q1, q2, bs.cpu().long()), y)
 
 
+def test_layer_without_tokens():
+    from gmm_b200.int8 import quantize_experts
+    from gmm_b200.moe import moe_forward_int8
+    x, logits, w1, w2 = (t.cuda() for t in layer(T=4))
+    q1, q2 = quantize_experts(w1), quantize_experts(w2)
+    out = moe_forward_int8(x[:0], logits[:0], q1, q2, k=2)
+    assert out.shape == (0, 256) and out.dtype == x.dtype
+
+
+def test_every_token_to_one_expert(tile):
+    """Device sizes chosen as for few rows an expert, all of them on one."""
+    from gmm_b200.int8 import gmm_int8_dev
+    bs = [0] * 40 + [500] + [0] * 23
+    p = problem(bs, 96, 48, seed=12)
+    got = gmm_int8_dev(*cuda(*p), torch.tensor(bs, dtype=torch.int32, device="cuda"), out_dtype=torch.float32)
+    check(got, exact(*p, bs), 3)
+
+
+def test_concurrent_host_threads():
+    """Calls from four host threads on streams of their own, with different kernels each."""
+    import threading
+    from gmm_b200.int8 import gmm_int8, quantize_rows
+    jobs = [problem(bs, 272, 136, seed=20 + i) + (bs,) for i, bs in enumerate(([3, 1, 9], [200, 0, 70], [900, 500], [16] * 30))]
+    want = [exact(*j[:4], j[4]) for j in jobs]
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            d = cuda(*jobs[i][:4])
+            x = rows_of(50 + i, 400, torch.bfloat16, seed=i)
+            for _ in range(20):
+                got = gmm_int8(*d, torch.tensor(jobs[i][4]), out_dtype=torch.float32)
+                q, s = quantize_rows(x.cuda())
+                torch.cuda.current_stream().synchronize()
+                wq, ws = spec_quantize(x)
+                if not (torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)):
+                    wrong.append(("quantize", i))
+                if ((got.double().cpu() - want[i]).abs() > want[i].abs() * 4 * H).any():
+                    wrong.append(("gmm", i))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_permute_without_rows():
     from gmm_b200.moe import permute
     g = torch.Generator().manual_seed(1)
