@@ -21,6 +21,10 @@
 // token rows on its N) for decode-shaped problems whose experts all have at
 // most 64 rows (choose_tile_kind).
 //
+// 8-bit operands (kind::i8, integer sums, scaled in the epilogue) run on the
+// 128-row and CTA-pair kernels too, and on gmm_stream_kernel.cuh for a few rows
+// an expert.
+//
 // A is addressed through one 2D tensor map over all T rows (a tile of expert
 // g starts at row off_g + 128 m); B through one 3D tensor map whose outer
 // coordinate is the expert.  No per-expert descriptors, no TMA multicast.

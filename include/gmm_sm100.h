@@ -57,12 +57,14 @@ const char* gmm_sm100_errstr(int status);
 /* Detail of the last failure on the calling thread (thread-local storage). */
 const char* gmm_sm100_last_error(void);
 
-/* Kernel family override for 16-bit problems.  No reference counterpart (the
+/* Kernel family override for 16-bit and 8-bit problems.  No reference counterpart (the
  * reference has one CUTLASS configuration per dtype).  GMM_TILE_AUTO picks
  * per problem (CTA-pair 256-row tiles when the non-empty experts average at
  * least 384 rows, swap-AB tiles when no expert has more than 64 rows, else
  * 128-row tiles); the others force one family (swap falls back to 128-row
- * tiles for the SwiGLU and expert-parallel epilogues).  Process-wide; the
+ * tiles for the SwiGLU and expert-parallel epilogues, and means the streaming
+ * kernel for 8-bit operands, which AUTO takes when no expert has more than 16
+ * rows and the weights are few).  Process-wide; the
  * initial value comes from the environment variable GMM_SM100_TILE
  * (128 / 256 / swap), read once.  Takes effect for plans made afterwards.
  * Returns the previous kind, or GMM_ERR_INVALID_ARGUMENT. */
@@ -203,8 +205,9 @@ int gmm_sm100_moe_unpermute(const void* y, const int32_t* dst_pos, const float* 
  * result is fp32, rounded once to out_dtype (fp32, bf16 or fp16).  swiglu: B
  * holds [gate rows | up rows], D is [num_tokens, dim_out / 2] and holds
  * silu(gate) * up of the scaled sums (bf16 / fp16).  Batch sizes, workspace,
- * streams and errors as in gmm_sm100_forward / gmm_sm100_forward_dev; A
- * scale that is NaN makes its row (column) NaN. */
+ * streams and errors as in gmm_sm100_forward / gmm_sm100_forward_dev; a call
+ * whose table needs the workspace is refused during stream capture.  A scale
+ * that is NaN makes its row (column) NaN. */
 int gmm_sm100_forward_int8(const int8_t* A, const float* scale_a, const int8_t* B, const float* scale_b,
                            const int64_t* batch_sizes, int64_t num_experts, int64_t num_tokens, int64_t dim,
                            int64_t dim_out, int out_dtype, int swiglu, void* D, void* workspace,
