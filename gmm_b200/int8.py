@@ -17,6 +17,7 @@ serving operators: no gradient flows through them.  No reference counterpart
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -24,10 +25,11 @@ import torch
 import gmm_b200
 
 
-def _ops():
+@functools.cache
+def _op(name: str):
     if not gmm_b200._HAS_C:
         raise RuntimeError("gmm_b200._C is not available. Build with `python -m gmm_b200.build`.")
-    return torch.ops.hopper_gmm_fwd
+    return getattr(torch.ops.hopper_gmm_fwd, name).default
 
 
 def quantize_rows(x: torch.Tensor, dst_pos: Optional[torch.Tensor] = None,
@@ -48,7 +50,7 @@ def quantize_rows(x: torch.Tensor, dst_pos: Optional[torch.Tensor] = None,
     """
     if out_rows is None:
         out_rows = x.shape[0] * (1 if dst_pos is None else dst_pos.shape[1])
-    return _ops().quantize_rows.default(x, dst_pos, out_rows)
+    return _op("quantize_rows")(x, dst_pos, out_rows)
 
 
 def quantize_experts(w: torch.Tensor, trans_b: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -85,7 +87,7 @@ def gmm_int8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
            ``silu(gate) * up`` of the scaled sums, ``[num_tokens, dim_out // 2]``
            (bf16 / fp16, ``dim_out`` a multiple of 16).
     """
-    return _ops().gmm_int8.default(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
+    return _op("gmm_int8")(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
 
 
 def gmm_int8_dev(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -95,4 +97,4 @@ def gmm_int8_dev(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scal
 
     ``a`` has capacity rows; the first ``sum(batch_sizes)`` are used and only
     those rows of the result are written."""
-    return _ops().gmm_int8_dev.default(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)
+    return _op("gmm_int8_dev")(a, a_scale, b, b_scale, batch_sizes, out_dtype, swiglu)

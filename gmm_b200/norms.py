@@ -15,6 +15,7 @@ second derivatives).  No reference counterpart.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -24,6 +25,7 @@ import gmm_b200
 _GATE_ACTS = {"none": 0, "tanh": 1, "sigmoid": 2}
 
 
+@functools.cache
 def _op():
     if not gmm_b200._HAS_C:
         raise RuntimeError("gmm_b200._C is not available. Build with `python -m gmm_b200.build`.")
