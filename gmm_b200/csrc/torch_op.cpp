@@ -17,9 +17,12 @@
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include "gmm_sm100.h"
@@ -375,6 +378,20 @@ const auto& post_norm_backward_op() {
 }
 
 // Gradients of post_norm: one node, whose backward is post_norm_backward.
+// A leaf that an eager graph still holds accumulates on that graph's stream. The legacy stream takes no event of a
+// captured one, and autograd meets that error on a thread where it ends the process: refused while it is an exception.
+void check_captured_leaves(const torch::autograd::variable_list& inputs) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = accumulator ? accumulator->stream() : std::nullopt;
+    TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(t.get_device()),
+                "post_norm: a graph made on the default stream still holds an input of this captured backward pass; "
+                "delete its outputs before the capture");
+  }
+}
+
 class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const OptTensor& y,
@@ -402,6 +419,7 @@ class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
     const OptTensor y = opt(saved[0]), next_weight = opt(saved[4]);
     const OptTensor dx_new = y ? opt(grads[0]) : OptTensor(), dh = next_weight ? opt(grads[1]) : OptTensor();
     if (!dx_new && !dh) return out;
+    check_captured_leaves(saved);
     const OptTensor weight = opt(saved[2]), gate = opt(saved[3]);
     const auto g = post_norm_backward_op().call(
         y, saved[1], weight, gate, next_weight, saved[5], dx_new, dh, ctx->saved_data["gate_act"].toInt(),

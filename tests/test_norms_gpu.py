@@ -408,6 +408,26 @@ def test_captured_forward_and_backward():
     assert all(torch.equal(out[k], want2[k]) for k in want2)
 
 
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    from gmm_b200.norms import post_norm
+    x, y, w = (torch.randn(*shape, device="cuda").requires_grad_() for shape in ((5, 16), (5, 16), (16,)))
+    alive = post_norm(y, x, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still holds an input"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(post_norm(y, x, w)[0].sum(), (x, y, w))
+    torch.cuda.synchronize()
+    # the eager graph is intact, and once it is gone the same step is captured
+    want = torch.autograd.grad(alive[0].sum(), (x, y, w))
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(post_norm(y, x, w)[0].sum(), (x, y, w))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_two_streams_at_once():
     cs = [cuda(inputs(700, 1000, torch.bfloat16, torch.float32, "full", seed=20 + i)) for i in range(2)]
     want = [train(c, "sigmoid") for c in cs]
