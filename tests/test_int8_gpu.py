@@ -554,3 +554,17 @@ def test_rows_past_32_bit_offsets():
     got = gmm_int8(q, scale, b.cuda(), sb.cuda(), torch.tensor([T]), out_dtype=torch.float32)
     check(got[-5:], exact(want_q, want_s, b, sb, [5]), 3)
     assert (got[:-5] == 0).all()
+
+
+def test_weights_past_32_bit_offsets(tile):
+    """The last of 140 experts lies beyond 2^31 bytes of weights."""
+    from gmm_b200.int8 import gmm_int8
+    experts, dim = 140, 4096
+    bs = [2] + [0] * (experts - 2) + [5]
+    a, sa, last, s_last = problem([7], dim, dim)
+    b = torch.zeros(experts, dim, dim, dtype=torch.int8, device="cuda")
+    sb = torch.ones(experts, dim, device="cuda")
+    b[-1], sb[-1] = last[0].cuda(), s_last[0].cuda()
+    got = gmm_int8(a.cuda(), sa.cuda(), b, sb, torch.tensor(bs), out_dtype=torch.float32)
+    assert (got[:2] == 0).all()
+    check(got[2:], exact(a[2:], sa[2:], last, s_last, [5]), 3)
