@@ -1279,11 +1279,14 @@ bool stream_fits(int64_t blocks, int64_t N) { return blocks <= INT32_MAX / (N / 
 // streaming kernel: it starts sooner and spreads small problems over every SM,
 // the 128-row tiles keep more of a long stream in flight.  One B200, bf16 out,
 // us, 8 rows an expert, streaming against 128-row tiles:
-//    2 x 768 x 2048 (3 MB)       5.9   9.4     64 x 768 x 2048 (101 MB)  24.9  25.5
-//    8 x 2048 x 1536 (25 MB)    10.5  17.4    128 x 768 x 2048 (201 MB)  42.2  40.2
-//    4 x 7168 x 4096 (117 MB)   26.5  32.2      8 x 7168 x 4096 (235 MB) 47.5  44.2
-//   32 x 768 x 2048 (50 MB)     14.8  17.0     64 x 2048 x 1536 (201 MB) 44.4  42.5
-constexpr double kStreamBytes = 1e8;
+//    2 x 768 x 2048 (3 MB)       5.9   9.4     64 x 768 x 2048 (101 MB)  24.7  25.9
+//    8 x 2048 x 1536 (25 MB)    10.5  17.4     96 x 768 x 2048 (151 MB)  33.8  34.6
+//    4 x 7168 x 4096 (117 MB)   27.6  33.5      5 x 7168 x 4096 (147 MB) 41.8  35.7
+//   32 x 768 x 2048 (50 MB)     14.8  17.0    128 x 768 x 2048 (201 MB)  42.2  40.2
+//   40 x 2048 x 1536 (126 MB)   29.4  32.8     64 x 2048 x 1536 (201 MB) 44.4  42.5
+// With 16 rows an expert the token rows cost as much as the weights:
+//   64 x 768 x 2048             29.2  26.8     40 x 2048 x 1536          30.2  32.9
+constexpr double kStreamBytes = 1.3e8;
 bool stream_pays(int64_t live, int64_t K, int64_t N) {
   return static_cast<double>(live) * static_cast<double>(K) * static_cast<double>(N) <= kStreamBytes;
 }
