@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
   ring.input(2, p.dxn, sizeof(T), p.dxn ? D : 0, pitch);
   ring.input(3, p.dh, sizeof(T), p.dh ? D : 0, pitch);
   ring.input(4, p.gate, p.gate_f32 ? 4 : sizeof(T), kMode == kFullGate ? D : 0, pitch);
-  ring.start(smem, slots, p.rows);
+  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode, sizeof(T), p.gate_f32));
   if (threadIdx.x < 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][(i & 1) * 32 + threadIdx.x] = 0.f;

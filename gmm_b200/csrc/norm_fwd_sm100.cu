@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
   ring.input(0, p.x, sizeof(T), D, D);
   ring.input(1, p.y, sizeof(T), kMode == kPreNorm ? 0 : D, D);
   ring.input(2, p.gate, p.gate_f32 ? 4 : sizeof(T), kMode == kFullGate ? D : 0, D);
-  ring.start(smem, slots, p.rows);
+  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode, sizeof(T), p.gate_f32));
   if (threadIdx.x < 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][i & 1][threadIdx.x] = 0.f;

@@ -387,12 +387,20 @@ int mode_of(const NormParams& p) {
   return !p.y ? kPreNorm : (p.gate_mode == GMM_GATE_MODE_FULL ? kFullGate : kSharedGate);
 }
 
+// Bytes of a slot behind an fp32 gate's row beside 16-bit rows off the word:
+// the kernels read it in units of two words, the last of which may end one
+// word past the row's last.
+__host__ __device__ constexpr uint32_t gate_pad(int layout, int mode, int es, int gate_f32) {
+  return layout == kShifted && mode == kFullGate && es == 2 && gate_f32 ? 16 : 0;
+}
+
 // Bytes of a slot that holds `inputs` rows of the data type and, with a gate
 // per element, one of the gate's.
 size_t slot_bytes(const NormParams& p, int es, int layout, int inputs) {
   const bool whole = layout == kWhole;
   const uint32_t gate = p.gate_mode == GMM_GATE_MODE_FULL ? p.dim * (p.gate_f32 ? 4 : es) : 0;
-  return static_cast<size_t>(row_pitch(p.dim * es, whole)) * inputs + (gate ? row_pitch(gate, whole) : 0);
+  return static_cast<size_t>(row_pitch(p.dim * es, whole)) * inputs + (gate ? row_pitch(gate, whole) : 0) +
+         gate_pad(layout, mode_of(p), es, p.gate_f32);
 }
 
 bool on(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

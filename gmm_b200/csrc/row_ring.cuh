@@ -144,14 +144,15 @@ struct RowRing {
     pitch_bytes[i] = static_cast<long long>(pitch) * elem;
   }
 
-  // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  The
-  // caller synchronises the block before the first wait.
-  __device__ __forceinline__ void start(uint8_t* mem, int n, long long num_rows) {
+  // Shared memory: slots * slot_bytes of rows, then one barrier a slot.  `pad`:
+  // bytes of a slot behind its last input's row.  The caller synchronises the
+  // block before the first wait.
+  __device__ __forceinline__ void start(uint8_t* mem, int n, long long num_rows, uint32_t pad = 0) {
     smem = mem;
     slots = n;
     rows = num_rows;
     dead = false;
-    slot_bytes = 0;
+    slot_bytes = pad;
     uint32_t least = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < kInputs; ++i) {
