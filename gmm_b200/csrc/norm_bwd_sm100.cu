@@ -13,7 +13,11 @@ namespace {
 // kWide: rows wider than the registers hold, in column windows of D elements
 // of rows `pitch` apart, each by a launch of its own: first every window's part
 // of the four sums, then its gradients from all windows' sums.
-template <typename T, int kLayout, int kE, int kMode, bool kWide>
+//
+// kNext: h has a gradient.  Without one the residual has no part in any
+// gradient (dx = dx', and of the four sums only A1 is left), and it is not
+// read: zeros times an infinity in it would be NaN.
+template <typename T, int kLayout, int kE, int kMode, bool kWide, bool kNext>
 __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const NormParams p, int slots) {
   constexpr int V = kUnit<T, kLayout>;
   // A thread works on groups of kG elements: one unit, or two of one element.
@@ -24,10 +28,10 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
   const int D = p.dim;
   RowRing<5, kLayout == kWhole> ring;
   const int pitch = kWide ? p.pitch : D;
-  ring.input(0, p.x, sizeof(T), D, pitch);
+  ring.input(0, p.x, sizeof(T), kNext ? D : 0, pitch);
   ring.input(1, p.y, sizeof(T), kMode == kPreNorm ? 0 : D, pitch);
   ring.input(2, p.dxn, sizeof(T), p.dxn ? D : 0, pitch);
-  ring.input(3, p.dh, sizeof(T), p.dh ? D : 0, pitch);
+  ring.input(3, p.dh, sizeof(T), kNext ? D : 0, pitch);
   ring.input(4, p.gate, p.gate_f32 ? 4 : sizeof(T), kMode == kFullGate ? D : 0, pitch);
   ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode, sizeof(T), p.gate_f32));
   if (threadIdx.x < 32)
@@ -37,7 +41,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
   const Span<V, kLayout> span(D, pitch);
   const int units = span.units;
   float pw[kE], vo[kE], acc[kE], dv[kE];
-  row_params<T, V, kLayout, kE, kMode>(p, span, p.dh != nullptr, pw, vo);
+  row_params<T, V, kLayout, kE, kMode>(p, span, kNext, pw, vo);
   auto input = [&](int i, int slot, long long row) {
     return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
   };
@@ -57,7 +61,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
   int odd = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float ry = kMode == kPreNorm ? 0.f : p.rstd_y[row];
-    const float rx = p.dh ? p.rstd_x[row] : 0.f;
+    const float rx = kNext ? p.rstd_x[row] : 0.f;
     const float tok = kMode == kSharedGate ? token_gate<T>(p, row) : 1.f;
     ring.wait(slot, phase, row);
     const uint8_t *in_x = input(0, slot, row), *in_y = input(1, slot, row), *in_dx = input(2, slot, row),
@@ -65,7 +69,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     auto unit = [&](int g, int u) { return static_cast<int>(threadIdx.x + (g * kU + u) * blockDim.x); };
     const Both to_x(kMode == kFullGate ? ry : ry * tok);
     // Of a group's elements: y, Q (times act(g) with a gate per element, which
-    // `a` returns), x', u = dh (v + o), dh.  Zeros past the row's end.
+    // `a` returns), x', u = dh (v + o), dh.  Zeros past the row's end; x', u
+    // and dh only with kNext.
     auto read = [&](int g, float (&y)[kG], float (&q)[kG], float (&a)[kG], float (&x)[kG], float (&u)[kG],
                     float (&dh)[kG]) {
 #pragma unroll
@@ -73,14 +78,9 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
         const int c = unit(g, k);
         const bool in = V > 1 || c < units;
         const auto& own = mask[g * kU + k];
-        read_unit_or_0<T, V>(in_x, c, in, own, x + k * V);
+        if constexpr (kNext) read_unit_or_0<T, V>(in_x, c, in, own, x + k * V);
         if constexpr (kMode != kPreNorm) read_unit_or_0<T, V>(in_y, c, in, own, y + k * V);
-        if (p.dh) {
-          read_unit_or_0<T, V>(in_dh, c, in, own, dh + k * V);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) dh[k * V + j] = 0.f;
-        }
+        if constexpr (kNext) read_unit_or_0<T, V>(in_dh, c, in, own, dh + k * V);
         if constexpr (kMode == kFullGate) {
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
@@ -95,9 +95,9 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
         if constexpr (kMode != kPreNorm) {
           mul2(q + j, y + j, pw + g * kG + j);
           if constexpr (kMode == kFullGate) mul2(q + j, q + j, a + j);
-          fma2(x + j, q + j, to_x, x + j);
+          if constexpr (kNext) fma2(x + j, q + j, to_x, x + j);
         }
-        mul2(u + j, dh + j, vo + g * kG + j);
+        if constexpr (kNext) mul2(u + j, dh + j, vo + g * kG + j);
       }
     };
     auto read_dx = [&](int g, float (&d)[kG]) {
@@ -123,11 +123,13 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
         if constexpr (kMode != kPreNorm) read_dx(g, d);
 #pragma unroll
         for (int j = 0; j < kG; j += 2) {
-          fma2(s2[0], u + j, x + j, s2[0]);
+          if constexpr (kNext) fma2(s2[0], u + j, x + j, s2[0]);
           if constexpr (kMode != kPreNorm) {
             fma2(s2[1], q + j, d + j, s2[1]);
-            fma2(s2[2], q + j, u + j, s2[2]);
-            fma2(s2[3], q + j, x + j, s2[3]);
+            if constexpr (kNext) {
+              fma2(s2[2], q + j, u + j, s2[2]);
+              fma2(s2[3], q + j, x + j, s2[3]);
+            }
           }
         }
       }
@@ -152,8 +154,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     }
     const bool results = !kWide || p.phase == 2;
     if (kWide && !results && threadIdx.x == 0) p.sums[p.window * p.rows + row] = make_float4(s[0], s[1], s[2], s[3]);
-    const float cx = rx * rx * (s[0] * inv_d) * rx;       // dx = dx' + r(x') u - cx x'
-    const float qdx = ry * (s[1] + rx * s[2] - cx * s[3]);  // sum of s (w + o) yh [act(g)] dx
+    const float cx = kNext ? rx * rx * (s[0] * inv_d) * rx : 0.f;                   // dx = dx' + r(x') u - cx x'
+    const float qdx = kNext ? ry * (s[1] + rx * s[2] - cx * s[3]) : ry * s[1];  // sum of s (w + o) yh [act(g)] dx
     const float m = qdx * inv_d * tok;                    // mean(t yh)
     if (results && (!kWide || p.window == 0) && kMode == kSharedGate && p.gate_mode == kGateToken && threadIdx.x == 0) {
       const float d = qdx * act_slope(tok, p.act);
@@ -169,13 +171,15 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
       float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG];
       read(g, y, q, a, x, u, dh);
       read_dx(g, d);
+      if constexpr (kNext) {
 #pragma unroll
-      for (int j = 0; j < kG; j += 2) {
-        const int e = g * kG + j;
-        fma2(d + j, u + j, r2, d + j);
-        fma2(d + j, x + j, neg_cx, d + j);  // dx
-        mul2(x + j, x + j, r2);
-        fma2(dv + e, dh + j, x + j, dv + e);
+        for (int j = 0; j < kG; j += 2) {
+          const int e = g * kG + j;
+          fma2(d + j, u + j, r2, d + j);
+          fma2(d + j, x + j, neg_cx, d + j);  // dx
+          mul2(x + j, x + j, r2);
+          fma2(dv + e, dh + j, x + j, dv + e);
+        }
       }
 #pragma unroll
       for (int k = 0; k < kU; ++k) {
@@ -250,14 +254,14 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) {
         if (kMode != kPreNorm) write_unit<float, 4>(part, c * (V / 4) + q, acc + i * V + 4 * q);
-        if (p.dh) write_unit<float, 4>(part + slice, c * (V / 4) + q, dv + i * V + 4 * q);
+        if (kNext) write_unit<float, 4>(part + slice, c * (V / 4) + q, dv + i * V + 4 * q);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (!span.has(c, j)) continue;
         if (kMode != kPreNorm) part[span.col(c, j)] = acc[i * V + j];
-        if (p.dh) part[slice + span.col(c, j)] = dv[i * V + j];
+        if (kNext) part[slice + span.col(c, j)] = dv[i * V + j];
       }
     }
   }
@@ -317,10 +321,10 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const ReduceParams p)
   store(p.dw, p.w_f32, s);
 }
 
-template <typename T, int kLayout, int kMode, bool kWide>
+template <typename T, int kLayout, int kMode, bool kWide, bool kNext>
 cudaError_t launch_bwd_ring(const NormParams& p, const RingShape& r, int blocks, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  auto kernel = norm_bwd_ring_kernel<T, kLayout, 16, kMode, kWide>;
+  auto kernel = norm_bwd_ring_kernel<T, kLayout, 16, kMode, kWide, kNext>;
   const cudaError_t e = allow_smem(kernel, done);
   if (e != cudaSuccess) return e;
   kernel<<<blocks, r.threads, r.smem, s>>>(p, r.slots);
@@ -367,12 +371,16 @@ BwdSpace bwd_space(int64_t rows, int dim, int sms) {
 
 template <typename T, int kLayout, bool kWide>
 cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
-  const int inputs = 1 + (p.y ? 1 : 0) + (p.dxn ? 1 : 0) + (p.dh ? 1 : 0);
+  const int inputs = (p.y ? 1 : 0) + (p.dxn ? 1 : 0) + (p.dh ? 2 : 0);  // x is read where dh is
   const RingShape r = ring_shape(l.span, 16, kBwdThreadsSm, slot_bytes(p, sizeof(T), kLayout, inputs));
   switch (mode_of(p)) {
-    case kPreNorm: return launch_bwd_ring<T, kLayout, kPreNorm, kWide>(p, r, blocks, s);
-    case kSharedGate: return launch_bwd_ring<T, kLayout, kSharedGate, kWide>(p, r, blocks, s);
-    default: return launch_bwd_ring<T, kLayout, kFullGate, kWide>(p, r, blocks, s);
+    case kPreNorm: return launch_bwd_ring<T, kLayout, kPreNorm, kWide, true>(p, r, blocks, s);
+    case kSharedGate:
+      return p.dh ? launch_bwd_ring<T, kLayout, kSharedGate, kWide, true>(p, r, blocks, s)
+                  : launch_bwd_ring<T, kLayout, kSharedGate, kWide, false>(p, r, blocks, s);
+    default:
+      return p.dh ? launch_bwd_ring<T, kLayout, kFullGate, kWide, true>(p, r, blocks, s)
+                  : launch_bwd_ring<T, kLayout, kFullGate, kWide, false>(p, r, blocks, s);
   }
 }
 

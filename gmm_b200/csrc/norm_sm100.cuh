@@ -21,6 +21,7 @@
 // Q = s act(g) (w + o) y:
 //   C = sum u x',  A1 = sum Q dx',  A2 = sum Q u,  B = sum Q x'
 //   c = r(x')^2 C / D,   sum t yh = r(y) (A1 + r(x') A2 - c r(x') B).
+// Without dh: dx = dx', sum t yh = r(y) A1, and x is not read.
 // Everything is held in fp32 and rounded once, on store.  Rows are walked by
 // blocks in a fixed order and parameter gradients added up per block, then
 // over blocks in order, so results do not change from run to run.

@@ -260,7 +260,8 @@ int gmm_sm100_post_norm(const void* y, const void* x, const void* weight, const 
                         float* rstd_y, float* rstd_x, void* stream);
 
 /* Its gradients, from dx_new and dh (either may be NULL, not both; dh NULL
- * leaves dnext_weight unwritten).  dy and dx are [rows, dim] of dtype; dweight,
+ * leaves dnext_weight unwritten and copies dx_new to dx: x has no part in the
+ * gradients then).  dy and dx are [rows, dim] of dtype; dweight,
  * dnext_weight and dgate have the types and shapes of weight, next_weight and
  * gate, summed in fp32 in a fixed order.  y NULL as in gmm_sm100_post_norm. */
 int gmm_sm100_post_norm_backward(const void* y, const void* x, const void* weight, const void* gate,
