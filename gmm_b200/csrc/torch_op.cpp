@@ -16,6 +16,7 @@
 //     time (hopper_gmm_forward.cu:442-446).
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -377,7 +378,18 @@ const auto& post_norm_backward_op() {
   return op;
 }
 
-// Gradients of post_norm: one node, whose backward is post_norm_backward.
+// The norms have no forward-mode derivative: a dual tensor's tangent would be dropped without a word.
+void refuse_forward_gradients(std::initializer_list<const at::Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                "post_norm has no forward-mode derivative (torch.func.jvp, torch.autograd.forward_ad)");
+}
+const at::Tensor& or_undefined(const OptTensor& t) {
+  static const at::Tensor none;
+  return t ? *t : none;
+}
+
 // A leaf that an eager graph still holds accumulates on that graph's stream. The legacy stream takes no event of a
 // captured one, and autograd meets that error on a thread where it ends the process: refused while it is an exception.
 void check_captured_leaves(const torch::autograd::variable_list& inputs) {
@@ -392,6 +404,7 @@ void check_captured_leaves(const torch::autograd::variable_list& inputs) {
   }
 }
 
+// Gradients of post_norm: one node, whose backward is post_norm_backward.
 class PostNormGrad : public torch::autograd::Function<PostNormGrad> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const OptTensor& y,
@@ -439,6 +452,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> post_norm_autograd(
     const OptTensor& y, const at::Tensor& x, const OptTensor& weight, const OptTensor& gate,
     const OptTensor& next_weight, int64_t gate_act, double residual_scale, double eps, double weight_offset,
     bool keep) {
+  refuse_forward_gradients(
+      {&or_undefined(y), &x, &or_undefined(weight), &or_undefined(gate), &or_undefined(next_weight)});
   bool grad = x.requires_grad();
   for (const OptTensor* t : {&y, &weight, &gate, &next_weight}) grad = grad || (t->has_value() && (*t)->requires_grad());
   if (!grad || !at::GradMode::is_enabled()) {
@@ -456,6 +471,8 @@ std::vector<at::Tensor> post_norm_backward_autograd(const OptTensor& y, const at
                                                     double weight_offset) {
   // reached with gradients on only under create_graph
   TORCH_CHECK(!at::GradMode::is_enabled(), "post_norm has no second derivative (create_graph=True)");
+  refuse_forward_gradients({&or_undefined(y), &x, &or_undefined(weight), &or_undefined(gate),
+                            &or_undefined(next_weight), &stats, &or_undefined(dx_new), &or_undefined(dh)});
   at::AutoDispatchBelowADInplaceOrView below;
   return post_norm_backward_op().call(y, x, weight, gate, next_weight, stats, dx_new, dh, gate_act, residual_scale,
                                       weight_offset);

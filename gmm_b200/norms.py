@@ -9,8 +9,8 @@ A block ``f`` with RMS norms before and after it computes, for each row::
 
 with ``r(z) = 1 / sqrt(mean(z ** 2) + eps)`` over the last dimension and ``o``
 the ``weight_offset``.  :func:`gmm_b200.moe.moe_block` runs an expert layer
-between the two.  Both functions are differentiable (one backward kernel; no
-second derivatives).  A backward pass captured into a CUDA graph is refused
+between the two.  Both functions have gradients (one backward kernel); second
+and forward-mode derivatives are refused.  A backward pass captured into a CUDA graph is refused
 while a graph made on the default stream still holds one of the leaves given
 here.  No reference counterpart.
 """
