@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from gmm_b200 import capi
 from gmm_b200.int8 import gmm_int8, gmm_int8_dev, quantize_rows
@@ -159,6 +160,13 @@ def moe_forward_int8(x: torch.Tensor, router_logits: torch.Tensor, w_gate_up: Tu
     return unpermute(y, dst_pos, w)
 
 
+def _differentiated(t: torch.Tensor) -> bool:
+    if t.requires_grad and torch.is_grad_enabled():
+        return True
+    # the level first: outside one, which is where a serving call is, unpacking ten arguments costs 18 us
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def moe_block(x: torch.Tensor, h: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, k: int,
               post_weight: torch.Tensor, next_weight: Optional[torch.Tensor] = None,
               gate: Optional[torch.Tensor] = None, gate_act: str = "none", residual_scale: float = 1.0,
@@ -170,7 +178,16 @@ def moe_block(x: torch.Tensor, h: torch.Tensor, w_router: torch.Tensor, w_gate_u
     after that).  The router's logits are ``h @ w_router`` (``[dim, E]``); the
     expert weights are tensors (``moe_forward``) or ``quantize_experts`` pairs
     (``moe_forward_int8``).  Returns what :func:`gmm_b200.norms.post_norm` does:
-    the new residual stream, and with ``next_weight`` the next block's ``h``."""
+    the new residual stream, and with ``next_weight`` the next block's ``h``.
+
+    The expert layer has no backward pass, so an argument that requires a
+    gradient (or carries a forward-mode one) is refused: run the block under
+    ``torch.no_grad()``."""
+    for t in (x, h, w_router, w_gate_up, w_down, post_weight, next_weight, gate):
+        for part in (t,) if t is None or isinstance(t, torch.Tensor) else t:
+            if part is not None and _differentiated(part):
+                raise RuntimeError("moe_block has no backward pass through its expert layer, and an argument requires a "
+                                   "gradient; run it under torch.no_grad()")
     layer = moe_forward if isinstance(w_gate_up, torch.Tensor) else moe_forward_int8
     y = layer(h, torch.matmul(h, w_router), w_gate_up, w_down, k, renormalize=renormalize)
     return post_norm(y, x, post_weight, gate=gate, gate_act=gate_act, residual_scale=residual_scale,

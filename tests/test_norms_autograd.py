@@ -56,3 +56,45 @@ def test_plain_tensors_inside_a_dual_level_run():
         assert run(t)[0].shape == (6, 40)
         t["x"].requires_grad_()
         assert run(t)[1].requires_grad
+
+
+# ------------------------------------------------------------------ the block between the norms
+BLOCK = ("x", "h", "router", "gate_up", "down", "post", "next", "gate")
+
+
+def block_inputs(int8):
+    shapes = {"x": (6, 48), "h": (6, 48), "router": (48, 4), "post": (48,), "next": (48,), "gate": (48,)}
+    t = {k: torch.empty(s, dtype=torch.bfloat16, device="cuda") for k, s in shapes.items()}
+    if int8:
+        t["gate_up"] = (torch.empty(4, 64, 48, dtype=torch.int8, device="cuda"), torch.empty(4, 64, device="cuda"))
+        t["down"] = (torch.empty(4, 48, 32, dtype=torch.int8, device="cuda"), torch.empty(4, 48, device="cuda"))
+    else:
+        t["gate_up"] = torch.empty(4, 48, 64, dtype=torch.bfloat16, device="cuda")
+        t["down"] = torch.empty(4, 32, 48, dtype=torch.bfloat16, device="cuda")
+    return t
+
+
+def block(t):
+    from gmm_b200.moe import moe_block
+    return moe_block(t["x"], t["h"], t["router"], t["gate_up"], t["down"], 2, t["post"], next_weight=t["next"], gate=t["gate"])
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("which", BLOCK)
+def test_a_block_refuses_gradients_it_would_drop(which, int8):
+    """Its expert layer keeps no graph, while the norm after it would: a gradient from it would lack the experts' part."""
+    with FakeTensorMode():
+        t = block_inputs(int8)
+        (t[which][1] if isinstance(t[which], tuple) else t[which]).requires_grad_()
+        t["down"] = list(t["down"]) if int8 else t["down"]  # a pair is any sequence of two
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            block(t)
+
+
+@pytest.mark.parametrize("which", BLOCK)
+def test_a_block_refuses_forward_gradients(which):
+    with FakeTensorMode(), torch.no_grad(), fwAD.dual_level():
+        t = block_inputs(False)
+        t[which] = fwAD.make_dual(t[which], torch.empty_like(t[which]))
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            block(t)
