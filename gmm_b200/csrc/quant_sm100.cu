@@ -225,22 +225,36 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const QuantParams p
   if (threadIdx.x < p.k && place >= 0) p.scales[place] = rs.scale;
 }
 
+// Blocks of the ring kernel on one SM, their row slots and dynamic shared
+// memory: as many blocks as threads and memory allow with two slots each, and
+// up to four slots in what is left, within what one block may have (two fit at
+// every width).  Besides its dynamic part a block takes its static scratch and
+// the system's, 1536 bytes.
+struct QuantShape {
+  int threads, resident, slots, smem;
+};
+QuantShape quant_shape(int dim, int dim_padded, int es, bool vec) {
+  QuantShape r;
+  r.threads = threads_for((dim_padded / 8 + kRingChunks - 1) / kRingChunks);
+  const int slot = static_cast<int>(row_pitch(dim * es, vec)) + 8, staged = 2 * dim_padded, extra = 1536;
+  r.resident = std::max(1, std::min({16, 1024 / r.threads, kRingBytes / (staged + extra + 2 * slot)}));
+  const int most = std::min(kRingBytes / r.resident - extra, kRingBlockBytes);
+  r.slots = std::max(2, std::min(4, (most - staged) / slot));
+  r.smem = staged + r.slots * slot;
+  return r;
+}
+
 template <typename T, bool kVec>
 cudaError_t launch(const QuantParams& p, int sms, cudaStream_t s) {
   const int chunks = p.dim_padded / 8;
   if (p.dim <= kMaxRingDim && p.dim > 0) {
-    // As many blocks as threads and shared memory allow with two slots each,
-    // and up to four slots in what is left (two fit at every width).
-    const int threads = threads_for((chunks + kRingChunks - 1) / kRingChunks);
-    const int slot = static_cast<int>(row_pitch(p.dim * sizeof(T), kVec)) + 8, fixed = 2 * p.dim_padded + 1024 + 512;
-    const int resident = std::max(1, std::min({16, 1024 / threads, kRingBytes / (fixed + 2 * slot)}));
-    const int slots = std::max(2, std::min(4, (kRingBytes / resident - fixed) / slot));
+    const QuantShape r = quant_shape(p.dim, p.dim_padded, sizeof(T), kVec);
     static std::atomic<unsigned long long> done{0};
     auto kernel = quantize_ring_kernel<T, kVec>;
     const cudaError_t e = allow_smem(kernel, done);
     if (e != cudaSuccess) return e;
-    const int grid = static_cast<int>(std::min<long long>(p.rows, static_cast<long long>(sms) * resident));
-    kernel<<<grid, threads, 2 * p.dim_padded + slots * slot, s>>>(p, slots);
+    const int grid = static_cast<int>(std::min<long long>(p.rows, static_cast<long long>(sms) * r.resident));
+    kernel<<<grid, r.threads, r.smem, s>>>(p, r.slots);
     return cudaSuccess;
   }
   const unsigned grid = static_cast<unsigned>(p.rows);

@@ -174,6 +174,7 @@ struct RowRing {
 
 // ------------------------------------------------------------------ host side
 constexpr int kRingBytes = 224 * 1024;  // shared memory of an SM the rings may take, over its resident blocks
+constexpr int kRingBlockBytes = kRingBytes - 2048;  // dynamic shared memory of one block, at most (allow_smem)
 
 inline int threads_for(int items) { return std::max(32, (items + 31) / 32 * 32); }
 
@@ -185,7 +186,7 @@ cudaError_t allow_smem(K kernel, std::atomic<unsigned long long>& done) {
   if (e != cudaSuccess) return e;
   const unsigned long long bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes - 2048);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBlockBytes);
   if (e == cudaSuccess) done.fetch_or(bit);
   return e;
 }

@@ -40,6 +40,53 @@ int main() {
 }
 """
 
+QUANT = r"""
+#include "quant_sm100.cu"
+using namespace gmm_sm100;
+// Every width and type of the quantiser's ring asks for no more than a block may have, and its blocks for no more than
+// an SM has (228 KB, with 1 KB of the system's and under 512 bytes of static scratch a block).
+int main() {
+  for (int es : {2, 4})
+    for (bool vec : {false, true})
+      for (int dim = 1; dim <= kMaxRingDim; ++dim) {
+        if (vec && dim % 8) continue;
+        const QuantShape r = quant_shape(dim, (dim + 15) / 16 * 16, es, vec);
+        if (r.smem > kRingBlockBytes || r.slots < 2 || r.resident * (r.smem + 1024 + 512) > 228 * 1024)
+          return std::printf("dim %d es %d vec %d: %d blocks of %d bytes\n", dim, es, vec, r.resident, r.smem), 1;
+      }
+  return 0;
+}
+"""
+
+NORM = r"""
+#include "norm_sm100.cuh"
+using namespace gmm_sm100;
+// The same of the norms: rows of one to five inputs, the last an fp32 gate's where there is one.
+int main() {
+  for (int es : {2, 4})
+    for (int dim = 1; dim <= kMaxNormDim; ++dim)
+      for (bool words : {false, true})
+        for (int inputs = 1; inputs <= 4; ++inputs)
+          for (int gate = 0; gate <= 1; ++gate)
+            for (bool backward : {false, true}) {
+              const RowLayout l = row_layout(dim, es, words);
+              if (l.span > (backward ? 8192 : kMaxNormDim) || (!backward && inputs > 2)) continue;
+              NormParams p = {};
+              p.y = &p;
+              p.dim = dim;
+              p.gate_mode = gate ? GMM_GATE_MODE_FULL : GMM_GATE_MODE_NONE;
+              p.gate_f32 = gate;
+              const int per = l.span <= 4096 && !backward ? 8 : 16;
+              const int threads = backward ? kBwdThreadsSm : l.span <= 4096 ? 1024 : l.span <= 8192 ? kFwdThreadsSm : 1024;
+              const RingShape r = ring_shape(l.span, per, threads, slot_bytes(p, es, l.layout, inputs));
+              if (r.slots < 1 || r.smem > kRingBlockBytes || r.resident * (r.smem + 1024 + 1024) > 228 * 1024)
+                return std::printf("dim %d es %d layout %d inputs %d: %d blocks of %d bytes\n", dim, es, l.layout, inputs,
+                                   r.resident, r.smem), 1;
+            }
+  return 0;
+}
+"""
+
 
 def run(tmp_path, source):
     nvcc = "/usr/local/cuda/bin/nvcc"
@@ -56,3 +103,11 @@ def run(tmp_path, source):
 
 def test_a_slot_holds_the_words_its_gate_is_read_in(tmp_path):
     run(tmp_path, GATE)
+
+
+def test_the_quantisers_ring_fits_at_every_width(tmp_path):
+    run(tmp_path, QUANT)
+
+
+def test_the_norms_ring_fits_at_every_width(tmp_path):
+    run(tmp_path, NORM)
