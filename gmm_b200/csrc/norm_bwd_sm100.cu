@@ -20,6 +20,7 @@ namespace {
 template <typename T, int kLayout, int kE, int kMode, bool kWide, bool kNext>
 __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const NormParams p, int slots) {
   constexpr int V = kUnit<T, kLayout>;
+  using G = GateOf<T, kMode>;  // of a gate per element
   // A thread works on groups of kG elements: one unit, or two of one element.
   constexpr int kU = V == 1 ? 2 : 1, kG = V * kU, kGroups = kE / kG;
   static_assert(kBwdThreadsSm <= 16 * 32, "block_sum4");
@@ -32,8 +33,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
   ring.input(1, p.y, sizeof(T), kMode == kPreNorm ? 0 : D, pitch);
   ring.input(2, p.dxn, sizeof(T), p.dxn ? D : 0, pitch);
   ring.input(3, p.dh, sizeof(T), kNext ? D : 0, pitch);
-  ring.input(4, p.gate, p.gate_f32 ? 4 : sizeof(T), kMode == kFullGate ? D : 0, pitch);
-  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode, sizeof(T), p.gate_f32));
+  ring.input(4, p.gate, sizeof(G), is_full(kMode) ? D : 0, pitch);
+  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode));
   if (threadIdx.x < 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][(i & 1) * 32 + threadIdx.x] = 0.f;
@@ -46,8 +47,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
   };
   // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
-  const bool wide_gate = kLayout == kShifted && kMode == kFullGate && sizeof(T) == 2 && p.gate_f32;
-  const int gate_words = wide_gate ? span.shift / 4 * 16 : 0;
+  const int gate_words = kLayout == kShifted && kMode == kFullGateF32 ? span.shift / 4 * 16 : 0;
   UnitMask<T, V, kLayout> mask[kE / V];
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) mask[i].set(span, threadIdx.x + i * blockDim.x);
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     const uint8_t *in_x = input(0, slot, row), *in_y = input(1, slot, row), *in_dx = input(2, slot, row),
                   *in_dh = input(3, slot, row), *in_g = input(4, slot, row) - gate_words;
     auto unit = [&](int g, int u) { return static_cast<int>(threadIdx.x + (g * kU + u) * blockDim.x); };
-    const Both to_x(kMode == kFullGate ? ry : ry * tok);
+    const Both to_x(is_full(kMode) ? ry : ry * tok);
     // Of a group's elements: y, Q (times act(g) with a gate per element, which
     // `a` returns), x', u = dh (v + o), dh.  Zeros past the row's end; x', u
     // and dh only with kNext.
@@ -81,20 +81,19 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
         if constexpr (kNext) read_unit_or_0<T, V>(in_x, c, in, own, x + k * V);
         if constexpr (kMode != kPreNorm) read_unit_or_0<T, V>(in_y, c, in, own, y + k * V);
         if constexpr (kNext) read_unit_or_0<T, V>(in_dh, c, in, own, dh + k * V);
-        if constexpr (kMode == kFullGate) {
+        if constexpr (is_full(kMode)) {
 #pragma unroll
           for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
-          if (in) read_param<T, V>(in_g, p.gate_f32, c, a + k * V);
+          if (in) read_param<G, V>(in_g, c, a + k * V);
           if (kLayout == kShifted) span.mask(c, a + k * V);
-#pragma unroll
-          for (int j = 0; j < V; ++j) a[k * V + j] = act_of(a[k * V + j], p.act);
+          act_of<sizeof(G) == 2, V>(a + k * V, p.act);
         }
       }
 #pragma unroll
       for (int j = 0; j < kG; j += 2) {
         if constexpr (kMode != kPreNorm) {
           mul2(q + j, y + j, pw + g * kG + j);
-          if constexpr (kMode == kFullGate) mul2(q + j, q + j, a + j);
+          if constexpr (is_full(kMode)) mul2(q + j, q + j, a + j);
           if constexpr (kNext) fma2(x + j, q + j, to_x, x + j);
         }
         if constexpr (kNext) mul2(u + j, dh + j, vo + g * kG + j);
@@ -191,7 +190,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
 #pragma unroll
         for (int j = 0; j < kG; j += 2) {
           const int e = g * kG + j;
-          if constexpr (kMode == kFullGate) {
+          if constexpr (is_full(kMode)) {
             float yh[2];
             mul2(yh, y + j, ry2);
 #pragma unroll
@@ -211,8 +210,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
           const int c = unit(g, k);
           if (V == 1 && c >= units) continue;
           span.write(dy_out, c, y + k * V);
-          if constexpr (kMode == kFullGate) {
-            if (p.gate_f32 && sizeof(T) == 2) {
+          if constexpr (is_full(kMode)) {
+            if constexpr (kMode == kFullGateF32) {
               float* out = static_cast<float*>(p.dgate_row) + row * pitch;
               if (V == 1 || span.partial(c)) {
 #pragma unroll
@@ -314,7 +313,8 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const ReduceParams p)
   }
   s *= p.scale;
   if (p.dgate) {
-    const float a = act_of(param1<T>(p.gate, p.gate_f32, col), p.act);
+    float a = param1<T>(p.gate, p.gate_f32, col);
+    act_of<false, 1>(&a, p.act);
     store(p.dgate, p.gate_f32, s * (param1<T>(p.w, p.w_f32, col) + p.offset) * act_slope(a, p.act));
     s *= a;
   }
@@ -373,14 +373,18 @@ template <typename T, int kLayout, bool kWide>
 cudaError_t bwd_ring_mode(const NormParams& p, const RowLayout& l, int blocks, cudaStream_t s) {
   const int inputs = (p.y ? 1 : 0) + (p.dxn ? 1 : 0) + (p.dh ? 2 : 0);  // x is read where dh is
   const RingShape r = ring_shape(l.span, 16, kBwdThreadsSm, slot_bytes(p, sizeof(T), kLayout, inputs));
-  switch (mode_of(p)) {
+  auto go = [&](auto mode) {
+    constexpr int kMode = decltype(mode)::value;
+    return p.dh ? launch_bwd_ring<T, kLayout, kMode, kWide, true>(p, r, blocks, s)
+                : launch_bwd_ring<T, kLayout, kMode, kWide, false>(p, r, blocks, s);
+  };
+  switch (mode_of(p, sizeof(T))) {
     case kPreNorm: return launch_bwd_ring<T, kLayout, kPreNorm, kWide, true>(p, r, blocks, s);
-    case kSharedGate:
-      return p.dh ? launch_bwd_ring<T, kLayout, kSharedGate, kWide, true>(p, r, blocks, s)
-                  : launch_bwd_ring<T, kLayout, kSharedGate, kWide, false>(p, r, blocks, s);
-    default:
-      return p.dh ? launch_bwd_ring<T, kLayout, kFullGate, kWide, true>(p, r, blocks, s)
-                  : launch_bwd_ring<T, kLayout, kFullGate, kWide, false>(p, r, blocks, s);
+    case kSharedGate: return go(std::integral_constant<int, kSharedGate>{});
+    case kFullGateF32:
+      if constexpr (sizeof(T) == 2) return go(std::integral_constant<int, kFullGateF32>{});
+      [[fallthrough]];
+    default: return go(std::integral_constant<int, kFullGate>{});
   }
 }
 

@@ -8,14 +8,15 @@ namespace {
 template <typename T, int kLayout, int kE, int kMode, int kThreads, int kBlocks>
 __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const NormParams p, int slots) {
   constexpr int V = kUnit<T, kLayout>, kUnits = kE / V;
+  using G = GateOf<T, kMode>;  // of a gate per element
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float scratch[2][2][kMaxWarps];  // by sum and by parity of the row
   const int D = p.dim;
   RowRing<3, kLayout == kWhole> ring;
   ring.input(0, p.x, sizeof(T), D, D);
   ring.input(1, p.y, sizeof(T), kMode == kPreNorm ? 0 : D, D);
-  ring.input(2, p.gate, p.gate_f32 ? 4 : sizeof(T), kMode == kFullGate ? D : 0, D);
-  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode, sizeof(T), p.gate_f32));
+  ring.input(2, p.gate, sizeof(G), is_full(kMode) ? D : 0, D);
+  ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode));
   if (threadIdx.x < 32)
 #pragma unroll
     for (int i = 0; i < 4; ++i) scratch[i >> 1][i & 1][threadIdx.x] = 0.f;
@@ -28,8 +29,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
     return smem + (kLayout == kShifted ? ring.word_at(slot, i) : ring.at(slot, i, row));
   };
   // An fp32 gate beside 16-bit rows: a unit is two words, and the row may start in the second.
-  const bool wide_gate = kLayout == kShifted && kMode == kFullGate && sizeof(T) == 2 && p.gate_f32;
-  const int gate_words = wide_gate ? span.shift / 4 * 16 : 0;
+  const int gate_words = kLayout == kShifted && kMode == kFullGateF32 ? span.shift / 4 * 16 : 0;
   UnitMask<T, V, kLayout> mask[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) mask[i].set(span, threadIdx.x + i * blockDim.x);
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
       }
 #pragma unroll
       for (int j = 0; j < kE; j += 2) fma2(sq, y + j, y + j, sq);
-      if constexpr (kMode == kFullGate) {  // y * act(g): the gate is not needed again
+      if constexpr (is_full(kMode)) {  // y * act(g): the gate is not needed again
         const auto* gs = input(2, slot, row) - gate_words;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
@@ -72,10 +72,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
           float g[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) g[j] = 0.f;
-          if (c < units) read_param<T, V>(gs, p.gate_f32, c, g);
+          if (c < units) read_param<G, V>(gs, c, g);
           if (kLayout == kShifted) span.mask(c, g);
+          act_of<sizeof(G) == 2, V>(g, p.act);
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[i * V + j] *= act_of(g[j], p.act);
+          for (int j = 0; j < V; ++j) y[i * V + j] *= g[j];
         }
       }
       const float ry = rsqrtf(block_sum(sq[0] + sq[1], scratch[0][odd]) * inv_d + p.eps);
@@ -157,7 +158,7 @@ cudaError_t fwd_ring(const NormParams& p, const RowLayout& l, int sms, cudaStrea
 //   8192 x 7168                     87              75
 template <typename T, int kLayout, int kMode>
 cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
-  if constexpr (kLayout != kShifted && kMode != kFullGate)
+  if constexpr (kLayout != kShifted && !is_full(kMode))
     if (l.span <= 4096) return fwd_ring<T, kLayout, 8, kMode, 512, 2>(p, l, sms, s);
   if (l.span <= 8192) return fwd_ring<T, kLayout, 16, kMode, kFwdThreadsSm, 1>(p, l, sms, s);
   return fwd_ring<T, kLayout, 16, kMode, 1024, 1>(p, l, sms, s);
@@ -165,9 +166,12 @@ cudaError_t fwd_ring_width(const NormParams& p, const RowLayout& l, int sms, cud
 
 template <typename T, int kLayout>
 cudaError_t fwd_ring_mode(const NormParams& p, const RowLayout& l, int sms, cudaStream_t s) {
-  switch (mode_of(p)) {
+  switch (mode_of(p, sizeof(T))) {
     case kPreNorm: return fwd_ring_width<T, kLayout, kPreNorm>(p, l, sms, s);
     case kSharedGate: return fwd_ring_width<T, kLayout, kSharedGate>(p, l, sms, s);
+    case kFullGateF32:
+      if constexpr (sizeof(T) == 2) return fwd_ring_width<T, kLayout, kFullGateF32>(p, l, sms, s);
+      [[fallthrough]];
     default: return fwd_ring_width<T, kLayout, kFullGate>(p, l, sms, s);
   }
 }

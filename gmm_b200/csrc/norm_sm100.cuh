@@ -80,11 +80,24 @@ struct NormParams {
   float scale, eps, offset;
 };
 
-__device__ __forceinline__ float act_of(float g, int act) {
-  // The sigmoid's fast exponential is within (2 |g| + 4) * 2^-24 of e^-g and
-  // its fast reciprocal within 2 * 2^-24; expf and a full division made a
-  // gate per element cost more than its rows' bytes (8191 x 6144 fp16: 111 us).
-  return act == GMM_GATE_TANH ? tanhf(g) : act == GMM_GATE_SIGMOID ? __fdividef(1.f, 1.f + __expf(-g)) : g;
+// g[j] = act(g[j]); one branch for all N, so that their exponentials overlap.
+// kFast: a 16-bit gate per element beside 16-bit rows.  There the sigmoid's
+// exponential and reciprocal are the fast ones, within 2 + 1.173 |g| and 2 ulp
+// (an ulp is up to 2^-23 of a value): together (9 + 2.35 |g|) * 2^-24, below a
+// half step of 16 bits for every g whose sigmoid they hold.  expf and a full
+// division (2 ulp and half an ulp) made such a gate cost more than its rows'
+// bytes (8191 x 6144 fp16: 111 us against 70); fp32 rows have twice the bytes
+// to hide them, and gates shared by rows or elements are few.
+template <bool kFast, int N>
+__device__ __forceinline__ void act_of(float* g, int act) {
+  if (act == GMM_GATE_TANH) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = tanhf(g[j]);
+  } else if (act == GMM_GATE_SIGMOID) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      g[j] = kFast ? __fdividef(1.f, 1.f + __expf(-g[j])) : 1.f / (1.f + expf(-g[j]));
+  }
 }
 // act'(g) from a = act(g)
 __device__ __forceinline__ float act_slope(float a, int act) {
@@ -137,8 +150,9 @@ __device__ __forceinline__ void block_sum4(float (&s)[4], float* scratch) {
 template <typename T>
 __device__ __forceinline__ float token_gate(const NormParams& p, long long row) {
   if (p.gate_mode != kGateToken) return 1.f;
-  const float g = p.gate_f32 ? static_cast<const float*>(p.gate)[row] : as_float(static_cast<const T*>(p.gate)[row]);
-  return act_of(g, p.act);
+  float g = p.gate_f32 ? static_cast<const float*>(p.gate)[row] : as_float(static_cast<const T*>(p.gate)[row]);
+  act_of<false, 1>(&g, p.act);
+  return g;
 }
 
 // ------------------------------------------------------------------ ring kernels
@@ -157,7 +171,11 @@ __device__ __forceinline__ float token_gate(const NormParams& p, long long row) 
 // 16384 x 4001 bf16, channel gate, forward, and forward and backward: kSingle
 // 160 and 600 us, kShifted 104 and 332; 4000 columns (kWhole) 88 and 231.
 enum Layout { kWhole = 0, kShifted = 1, kSingle = 2 };
-enum RingMode { kPreNorm = 0, kSharedGate = 1, kFullGate = 2 };  // no y | gate none, channel, token | gate per element
+// no y | gate none, channel, token | gate per element of the rows' type | of fp32 beside 16-bit rows
+enum RingMode { kPreNorm = 0, kSharedGate = 1, kFullGate = 2, kFullGateF32 = 3 };
+__host__ __device__ constexpr bool is_full(int mode) { return mode >= kFullGate; }
+template <typename T, int kMode>
+using GateOf = typename std::conditional<kMode == kFullGateF32, float, T>::type;
 
 template <typename T, int kLayout>
 constexpr int kUnit = kLayout == kSingle ? 1 : 16 / static_cast<int>(sizeof(T));
@@ -203,19 +221,21 @@ __device__ __forceinline__ void read_unit_or_0(const void* row, int c, bool in, 
   unpack_unit<T, V>(mask(r), f);
 }
 
-// Unit c of a parameter or gate row that is T or fp32.
+// Unit c (V elements) of a row of G: a gate's, or a parameter's.
+template <typename G, int V>
+__device__ __forceinline__ void read_param(const void* row, int c, float* f) {
+  if constexpr (V == 1) {
+    f[0] = as_float(static_cast<const G*>(row)[c]);
+  } else {
+    constexpr int kPer = 16 / static_cast<int>(sizeof(G));
+#pragma unroll
+    for (int q = 0; q < V / kPer; ++q) unpack16<G>(static_cast<const uint4*>(row)[c * (V / kPer) + q], f + kPer * q);
+  }
+}
 template <typename T, int V>
 __device__ __forceinline__ void read_param(const void* row, bool f32, int c, float* f) {
-  if (f32 && sizeof(T) == 2) {
-    if constexpr (V == 1) {
-      f[0] = static_cast<const float*>(row)[c];
-    } else {
-#pragma unroll
-      for (int q = 0; q < V / 4; ++q) unpack16<float>(static_cast<const uint4*>(row)[c * (V / 4) + q], f + 4 * q);
-    }
-  } else {
-    read_unit<T, V>(row, c, f);
-  }
+  if (f32 && sizeof(T) == 2) read_param<float, V>(row, c, f);
+  else read_param<T, V>(row, c, f);
 }
 
 template <typename T, int V>
@@ -334,13 +354,15 @@ __device__ __forceinline__ void row_params(const NormParams& p, const Span<V, kL
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
+    if constexpr (kMode == kSharedGate)
+      if (channel) act_of<false, V>(g + i * V, p.act);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const bool in = span.has(c, j);
       const int e = i * V + j;
       if (kMode != kPreNorm) {
         pw[e] = in ? (pw[e] + p.offset) * p.scale : 0.f;
-        if (kMode == kSharedGate && channel) pw[e] *= act_of(g[e], p.act);
+        if (kMode == kSharedGate && channel) pw[e] *= g[e];
       }
       vo[e] = in && with_v ? vo[e] + p.offset : 0.f;
     }
@@ -384,15 +406,17 @@ int blocks_for(int64_t rows, int64_t most, int period) {
   return static_cast<int>(std::max<int64_t>(period, most / period * period));
 }
 
-int mode_of(const NormParams& p) {
-  return !p.y ? kPreNorm : (p.gate_mode == GMM_GATE_MODE_FULL ? kFullGate : kSharedGate);
+int mode_of(const NormParams& p, int es) {
+  if (!p.y) return kPreNorm;
+  if (p.gate_mode != GMM_GATE_MODE_FULL) return kSharedGate;
+  return es == 2 && p.gate_f32 ? kFullGateF32 : kFullGate;
 }
 
 // Bytes of a slot behind an fp32 gate's row beside 16-bit rows off the word:
 // the kernels read it in units of two words, the last of which may end one
 // word past the row's last.
-__host__ __device__ constexpr uint32_t gate_pad(int layout, int mode, int es, int gate_f32) {
-  return layout == kShifted && mode == kFullGate && es == 2 && gate_f32 ? 16 : 0;
+__host__ __device__ constexpr uint32_t gate_pad(int layout, int mode) {
+  return layout == kShifted && mode == kFullGateF32 ? 16 : 0;
 }
 
 // Bytes of a slot that holds `inputs` rows of the data type and, with a gate
@@ -401,7 +425,7 @@ size_t slot_bytes(const NormParams& p, int es, int layout, int inputs) {
   const bool whole = layout == kWhole;
   const uint32_t gate = p.gate_mode == GMM_GATE_MODE_FULL ? p.dim * (p.gate_f32 ? 4 : es) : 0;
   return static_cast<size_t>(row_pitch(p.dim * es, whole)) * inputs + (gate ? row_pitch(gate, whole) : 0) +
-         gate_pad(layout, mode_of(p), es, p.gate_f32);
+         gate_pad(layout, mode_of(p, es));
 }
 
 bool on(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

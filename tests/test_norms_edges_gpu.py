@@ -1,9 +1,9 @@
-"""Norms where a gradient is finite beside an infinity."""
+"""Norms where a gradient is finite beside an infinity and where a gate saturates."""
 
 import pytest
 import torch
 
-from test_norms_gpu import check, cuda, formulas, inputs, train
+from test_norms_gpu import HALF_STEP, H, TINY, check, cuda, formulas, inputs, train
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,70 @@ def test_without_a_gradient_of_h_a_spoilt_y_leaves_dx():
     got = train(cuda(d), "none", 0.7)
     assert torch.equal(got["dx"].cpu(), d["dx"])
     assert got["dy"][1].isnan().all() and not got["dy"][0].isnan().any()
+
+
+# ------------------------------------------------------------------ gates
+# Rows of y = 1 with eps = 0 and a power of two elements have mean 1 exactly, so r(y) is 1 within rsqrtf's 2 ulp (4 h).
+GATES = [0.0, 0.3, 0.5, 1.0, 2.0, 3.3, 4.0, 6.7, 8.0, 10.0, 12.0, 14.1, 16.0, 20.0, 30.0]
+
+
+def gate_values(dtype, n):
+    g = torch.tensor([s * v for v in GATES for s in (1, -1)] + [float("inf"), float("-inf")])
+    spread = (torch.rand(n - g.numel(), generator=torch.Generator().manual_seed(41)) * 2 - 1) * 30
+    return torch.cat([g, spread]).to(dtype)
+
+
+def gate_exact(g, kind):
+    """act(g) and act'(g) in fp64, neither from the other by a difference."""
+    g = g.double()
+    if kind == "sigmoid":
+        e = torch.exp(-g.abs())
+        return torch.where(g >= 0, 1 / (1 + e), e / (1 + e)), e / (1 + e) ** 2
+    e = torch.exp(-2 * g.abs())
+    return torch.tanh(g), 4 * e / (1 + e) ** 2
+
+
+def gate_case(gate, dtype, gate_dtype, kind):
+    """x_new and dgate of rows of ones (x = 0, w = 1, dx' = 1): act(g), and D or T times act'(g) where g is shared."""
+    from gmm_b200.norms import post_norm
+    T, D = {"channel": (1, 1024), "token": (1024, 8), "full": (8, 1024)}[gate]
+    g = gate_values(gate_dtype, 1024)
+    shape = {"channel": (D,), "token": (T, 1), "full": (T, D)}[gate]
+    g = g.repeat(8).view(T, D) if gate == "full" else g.view(shape)
+    y = torch.ones(T, D, dtype=dtype, device="cuda", requires_grad=True)
+    x, w = torch.zeros(T, D, dtype=dtype, device="cuda"), torch.ones(D, device="cuda")
+    leaf = g.cuda().requires_grad_()
+    new = post_norm(y, x, w, gate=leaf, gate_act=kind, eps=0.0)
+    dg, = torch.autograd.grad(new, leaf, torch.ones_like(new))
+    a, da = gate_exact(g, kind)
+    return new, a.expand(T, D), dg, da * (D if gate == "token" else 1)
+
+
+def near(got, want, rel, what):
+    tol = want.abs() * (rel + HALF_STEP[got.dtype] * (1 + 2.0 ** -8)) + TINY[got.dtype]
+    off = (got.detach().double().cpu() - want).abs()
+    worst = (off / tol).argmax()
+    assert (off <= tol).all(), (what, float((off / tol).max()), int(worst))
+
+
+GATES_OF = pytest.mark.parametrize("gate", ["channel", "token", "full"])
+KINDS = pytest.mark.parametrize("kind", ["tanh", "sigmoid"])
+
+
+@GATES_OF
+@KINDS
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_act_of_fp32_gates(dtype, kind, gate):
+    """An fp32 gate beside rows of any type: act(g) within 14 h of its value at any |g|.  The exponential 2 ulp (4 h), the
+    sum, the quotient and a product h each, or tanhf 2 ulp; r(y) 4 h and three products."""
+    new, a, _, _ = gate_case(gate, dtype, torch.float32, kind)
+    near(new, a, 14 * H, "act")
+
+
+@GATES_OF
+@KINDS
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_act_of_16_bit_gates(dtype, kind, gate):
+    """The fast exponential of x is within 2 + 1.173 |x| ulp, 75 h at |x| = 30, the fast quotient 2 ulp, the rest as above."""
+    new, a, _, _ = gate_case(gate, dtype, dtype, kind)
+    near(new, a, 100 * H, "act")
