@@ -70,9 +70,9 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     const Both to_x(is_full(kMode) ? ry : ry * tok);
     // Of a group's elements: y, Q (times act(g) with a gate per element, which
     // `a` returns), x', u = dh (v + o), dh.  Zeros past the row's end; x', u
-    // and dh only with kNext.
+    // and dh only with kNext.  `slope` returns act'(g) if it is there.
     auto read = [&](int g, float (&y)[kG], float (&q)[kG], float (&a)[kG], float (&x)[kG], float (&u)[kG],
-                    float (&dh)[kG]) {
+                    float (&dh)[kG], float* slope) {
 #pragma unroll
       for (int k = 0; k < kU; ++k) {
         const int c = unit(g, k);
@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
           for (int j = 0; j < V; ++j) a[k * V + j] = 0.f;
           if (in) read_param<G, V>(in_g, c, a + k * V);
           if (kLayout == kShifted) span.mask(c, a + k * V);
-          act_of<sizeof(G) == 2, V>(a + k * V, p.act);
+          if (slope) act_of<sizeof(G) == 2, true, V>(a + k * V, p.act, slope + k * V);
+          else act_of<sizeof(G) == 2, false, V>(a + k * V, p.act);
         }
       }
 #pragma unroll
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
       for (int g = 0; g < kGroups; ++g) {
         if (V > 1 && unit(g, 0) >= units) continue;
         float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG];
-        read(g, y, q, a, x, u, dh);
+        read(g, y, q, a, x, u, dh, nullptr);
         if constexpr (kMode != kPreNorm) read_dx(g, d);
 #pragma unroll
         for (int j = 0; j < kG; j += 2) {
@@ -157,7 +158,9 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
     const float qdx = kNext ? ry * (s[1] + rx * s[2] - cx * s[3]) : ry * s[1];  // sum of s (w + o) yh [act(g)] dx
     const float m = qdx * inv_d * tok;                    // mean(t yh)
     if (results && (!kWide || p.window == 0) && kMode == kSharedGate && p.gate_mode == kGateToken && threadIdx.x == 0) {
-      const float d = qdx * act_slope(tok, p.act);
+      float g = token_value<T>(p, row), slope;
+      act_of<false, true, 1>(&g, p.act, &slope);
+      const float d = qdx * slope;
       if (p.gate_f32) static_cast<float*>(p.dgate_row)[row] = d;
       else static_cast<T*>(p.dgate_row)[row] = from_float<T>(d);
     }
@@ -167,8 +170,8 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       if (!results || (V > 1 && unit(g, 0) >= units)) continue;
-      float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG];
-      read(g, y, q, a, x, u, dh);
+      float y[kG], q[kG], a[kG], x[kG], u[kG], dh[kG], d[kG], dg[kG];  // dg: act'(g) first
+      read(g, y, q, a, x, u, dh, dg);
       read_dx(g, d);
       if constexpr (kNext) {
 #pragma unroll
@@ -186,7 +189,6 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
         if (V > 1 || c < units) span.write(dx_out, c, d + k * V);
       }
       if constexpr (kMode != kPreNorm) {
-        float dg[kG];
 #pragma unroll
         for (int j = 0; j < kG; j += 2) {
           const int e = g * kG + j;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kBwdThreadsSm) norm_bwd_ring_kernel(const Norm
             float yh[2];
             mul2(yh, y + j, ry2);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) dg[j + i] = pw[e + i] * yh[i] * d[j + i] * act_slope(a[j + i], p.act);
+            for (int i = 0; i < 2; ++i) dg[j + i] *= pw[e + i] * yh[i] * d[j + i];
             mul2(d + j, d + j, a + j);
             fma2(acc + e, d + j, yh, acc + e);
             mul2(d + j, d + j, ry2);
@@ -313,9 +315,9 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const ReduceParams p)
   }
   s *= p.scale;
   if (p.dgate) {
-    float a = param1<T>(p.gate, p.gate_f32, col);
-    act_of<false, 1>(&a, p.act);
-    store(p.dgate, p.gate_f32, s * (param1<T>(p.w, p.w_f32, col) + p.offset) * act_slope(a, p.act));
+    float a = param1<T>(p.gate, p.gate_f32, col), slope;
+    act_of<false, true, 1>(&a, p.act, &slope);
+    store(p.dgate, p.gate_f32, s * (param1<T>(p.w, p.w_f32, col) + p.offset) * slope);
     s *= a;
   }
   store(p.dw, p.w_f32, s);

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
           for (int j = 0; j < V; ++j) g[j] = 0.f;
           if (c < units) read_param<G, V>(gs, c, g);
           if (kLayout == kShifted) span.mask(c, g);
-          act_of<sizeof(G) == 2, V>(g, p.act);
+          act_of<sizeof(G) == 2, false, V>(g, p.act);
 #pragma unroll
           for (int j = 0; j < V; ++j) y[i * V + j] *= g[j];
         }

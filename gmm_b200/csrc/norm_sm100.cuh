@@ -80,28 +80,53 @@ struct NormParams {
   float scale, eps, offset;
 };
 
-// g[j] = act(g[j]); one branch for all N, so that their exponentials overlap.
-// kFast: a 16-bit gate per element beside 16-bit rows.  There the sigmoid's
-// exponential and reciprocal are the fast ones, within 2 + 1.173 |g| and 2 ulp
-// (an ulp is up to 2^-23 of a value): together (9 + 2.35 |g|) * 2^-24, below a
-// half step of 16 bits for every g whose sigmoid they hold.  expf and a full
-// division (2 ulp and half an ulp) made such a gate cost more than its rows'
-// bytes (8191 x 6144 fp16: 111 us against 70); fp32 rows have twice the bytes
-// to hide them, and gates shared by rows or elements are few.
-template <bool kFast, int N>
-__device__ __forceinline__ void act_of(float* g, int act) {
+// g[j] = act(g[j]) and, with kSlope, slope[j] = act'(g[j]); one branch for all
+// N, so that their exponentials overlap.  With e = exp(-|g|), r = 1 / (1 + e):
+//   sigmoid  r or e r by the sign of g, slope e r^2  (without kSlope from exp(-g) alone)
+//   tanh     slope 4 e r^2 with e = exp(-2 |g|)
+// Slopes from a (1 - a) or 1 - a^2 would lose a saturated gate's to the
+// rounding of a.
+//
+// kFast: a 16-bit gate per element beside 16-bit rows.  There exponential and
+// reciprocal are the fast ones, within 2 + 1.173 |x| and 2 ulp (an ulp is up to
+// 2^-23 of a value): the sigmoid (10 + 2.35 |g|) * 2^-24 and the slopes, twice
+// the reciprocal and twice the argument for tanh, below (20 + 4.7 |g|) * 2^-24,
+// less than a half step of 16 bits (results below 2^-126 may be 0).  expf
+// and a correctly rounded reciprocal made such a gate cost more than its rows'
+// bytes (8191 x 6144 fp16 forward: 111 us against 70); fp32 rows have twice the
+// bytes to hide them, and gates shared by rows or elements are few.
+template <bool kFast, bool kSlope, int N>
+__device__ __forceinline__ void act_of(float* g, int act, float* slope = nullptr) {
+  auto ratio = [](float x, float& e) {
+    e = kFast ? __expf(x) : expf(x);
+    return kFast ? __fdividef(1.f, 1.f + e) : __frcp_rn(1.f + e);
+  };
   if (act == GMM_GATE_TANH) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) g[j] = tanhf(g[j]);
+    for (int j = 0; j < N; ++j) {
+      if constexpr (kSlope) {
+        float e;
+        const float r = ratio(-2.f * fabsf(g[j]), e);
+        slope[j] = 4.f * (e * r) * r;
+      }
+      g[j] = tanhf(g[j]);
+    }
   } else if (act == GMM_GATE_SIGMOID) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      g[j] = kFast ? __fdividef(1.f, 1.f + __expf(-g[j])) : 1.f / (1.f + expf(-g[j]));
+    for (int j = 0; j < N; ++j) {
+      float e;
+      if constexpr (kSlope) {
+        const float r = ratio(-fabsf(g[j]), e), er = e * r;
+        slope[j] = er * r;
+        g[j] = g[j] >= 0.f ? r : er;
+      } else {
+        g[j] = ratio(-g[j], e);
+      }
+    }
+  } else if constexpr (kSlope) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) slope[j] = 1.f;
   }
-}
-// act'(g) from a = act(g)
-__device__ __forceinline__ float act_slope(float a, int act) {
-  return act == GMM_GATE_TANH ? 1.f - a * a : act == GMM_GATE_SIGMOID ? a * (1.f - a) : 1.f;
 }
 
 constexpr int kMaxWarps = 32;
@@ -146,12 +171,16 @@ __device__ __forceinline__ void block_sum4(float (&s)[4], float* scratch) {
   for (int j = 0; j < 4; ++j) s[j] = __shfl_sync(0xffffffffu, t, 8 * j);
 }
 
-// act(g) of a token gate's row, 1 for the others.
+// A token gate's row, and act(g) of it (1 for the other gates).
+template <typename T>
+__device__ __forceinline__ float token_value(const NormParams& p, long long row) {
+  return p.gate_f32 ? static_cast<const float*>(p.gate)[row] : as_float(static_cast<const T*>(p.gate)[row]);
+}
 template <typename T>
 __device__ __forceinline__ float token_gate(const NormParams& p, long long row) {
   if (p.gate_mode != kGateToken) return 1.f;
-  float g = p.gate_f32 ? static_cast<const float*>(p.gate)[row] : as_float(static_cast<const T*>(p.gate)[row]);
-  act_of<false, 1>(&g, p.act);
+  float g = token_value<T>(p, row);
+  act_of<false, false, 1>(&g, p.act);
   return g;
 }
 
@@ -355,7 +384,7 @@ __device__ __forceinline__ void row_params(const NormParams& p, const Span<V, kL
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if constexpr (kMode == kSharedGate)
-      if (channel) act_of<false, V>(g + i * V, p.act);
+      if (channel) act_of<false, false, V>(g + i * V, p.act);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const bool in = span.has(c, j);

@@ -111,3 +111,33 @@ def test_act_of_16_bit_gates(dtype, kind, gate):
     """The fast exponential of x is within 2 + 1.173 |x| ulp, 75 h at |x| = 30, the fast quotient 2 ulp, the rest as above."""
     new, a, _, _ = gate_case(gate, dtype, dtype, kind)
     near(new, a, 100 * H, "act")
+
+
+@GATES_OF
+@KINDS
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_slope_of_fp32_gates(dtype, kind, gate):
+    """act'(g) within 24 h of its value, however far the gate is saturated: the exponential 4 h, 1 + e and its square 3 h,
+    the quotients and products 3 h; r(y) 4 h, the products with pw, y and dx' 4 h, and the sum over equal elements of a
+    row 3 h (channel: one row)."""
+    _, _, dg, da = gate_case(gate, dtype, torch.float32, kind)
+    near(dg, da, 24 * H, "slope")
+
+
+@GATES_OF
+@KINDS
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_slope_of_16_bit_gates(dtype, kind, gate):
+    """The fast exponential of x is within 146 h for |x| = 60 (tanh's slope at |g| = 30), and the rest of the slope less than
+    40 h; the gradient's own half step (2^-11 and more) is above both."""
+    _, _, dg, da = gate_case(gate, dtype, dtype, kind)
+    near(dg, da, 200 * H, "slope")
+
+
+@GATES_OF
+@KINDS
+def test_no_slope_at_infinite_gates(gate, kind):
+    _, _, dg, _ = gate_case(gate, torch.float32, torch.float32, kind)
+    at = gate_values(torch.float32, 1024).isinf()
+    dg = dg.flatten()[:1024].cpu()
+    assert (dg[at] == 0).all() and not dg.isnan().any()
