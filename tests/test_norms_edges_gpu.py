@@ -1,4 +1,4 @@
-"""Norms where a gradient is finite beside an infinity and where a gate saturates."""
+"""Norms where a gradient is finite beside an infinity and where a gate saturates, and at the ends of their buffers."""
 
 import pytest
 import torch
@@ -141,3 +141,93 @@ def test_no_slope_at_infinite_gates(gate, kind):
     at = gate_values(torch.float32, 1024).isinf()
     dg = dg.flatten()[:1024].cpu()
     assert (dg[at] == 0).all() and not dg.isnan().any()
+
+
+# ------------------------------------------------------------------ the ends of the buffers
+GUARD = 512
+FILL = 0xA5
+
+
+class Guarded:
+    """Buffers between guard regions; an output starts `shift` bytes off a 16-byte word and ends with its last byte."""
+
+    def __init__(self):
+        self.made = []
+
+    def empty(self, shape, dtype, shift=0):
+        size = torch.empty(0, dtype=dtype).element_size()
+        n = size
+        for s in shape:
+            n *= s
+        raw = torch.full((GUARD + shift + n + GUARD,), FILL, dtype=torch.uint8, device="cuda")
+        self.made.append((raw, GUARD + shift, n))
+        view = raw[GUARD + shift: GUARD + shift + n]
+        return raw.data_ptr() + GUARD + shift, lambda: view.clone().view(dtype).view(shape)
+
+    def check(self):
+        torch.cuda.synchronize()
+        for i, (raw, at, n) in enumerate(self.made):
+            assert (raw[:at] == FILL).all(), ("before buffer", i)
+            assert (raw[at + n:] == FILL).all(), ("behind buffer", i)
+
+
+def code(t):
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[t]
+
+
+@pytest.mark.parametrize("off", [False, True])
+@pytest.mark.parametrize("gate,gate_dtype", [("none", None), ("channel", torch.float32), ("channel", None),
+                                             ("token", None), ("full", None), ("full", torch.float32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,D", [(1, 1), (300, 3), (700, 11), (5, 33), (400, 250), (160, 2050), (9, 4091), (3, 4096),
+                                 (151, 8195), (2, 16363), (3, 16384)])
+def test_nothing_is_written_outside(T, D, dtype, gate, gate_dtype, off):
+    """Forward and backward through the C entry points, every output and the workspace between guards; the results
+    are those of tensors of their own."""
+    from gmm_b200 import capi
+    lib = capi.load()
+    gate_dtype = gate_dtype or dtype
+    d = inputs(T, D, dtype, torch.float32, gate, seed=51)
+    if d["g"] is not None:
+        d["g"] = d["g"].to(gate_dtype)
+    c = cuda(d)
+    want = train(c, "tanh", 0.7)
+    mode = ["none", "channel", "token", "full"].index(gate if gate != "token" or D > 1 else "full")  # as post_norm reads the shapes
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    out = Guarded()
+    es = 4 if dtype == torch.float32 else 2
+    shift = es if off else 0
+    new, new_t = out.empty((T, D), dtype, shift)
+    h, h_t = out.empty((T, D), dtype, shift)
+    ry, _ = out.empty((T,), torch.float32)
+    rx, _ = out.empty((T,), torch.float32)
+    head = (T, D, code(dtype), 0, code(gate_dtype), mode, 1, 0.7)
+    rc = lib.gmm_sm100_post_norm(ptr(c["y"]), ptr(c["x"]), ptr(c["w"]), ptr(c["g"]), ptr(c["v"]), *head, 1e-6, 0.0, new, h,
+                                 ry, rx, None)
+    assert rc == 0, lib.gmm_sm100_last_error()
+    dy, dy_t = out.empty((T, D), dtype, shift)
+    dx, dx_t = out.empty((T, D), dtype, shift)
+    dw, dw_t = out.empty((D,), torch.float32)
+    dv, dv_t = out.empty((D,), torch.float32)
+    dg, dg_t = out.empty(tuple(d["g"].shape), gate_dtype, shift if gate_dtype == dtype else 0) if mode else (None, None)
+    size = lib.gmm_sm100_post_norm_backward_workspace_size(T, D)
+    ws, _ = out.empty((size,), torch.uint8)
+    rc = lib.gmm_sm100_post_norm_backward(ptr(c["y"]), ptr(c["x"]), ptr(c["w"]), ptr(c["g"]), ptr(c["v"]), ry, rx,
+                                          ptr(c["dx"]), ptr(c["dh"]), *head, 0.0, dy, dx, dw, dg, dv, ws, size, None)
+    assert rc == 0, lib.gmm_sm100_last_error()
+    out.check()
+    for k, t in (("new", new_t), ("h", h_t), ("dy", dy_t), ("dx", dx_t), ("dw", dw_t), ("dv", dv_t), ("dg", dg_t)):
+        if t is None:
+            continue
+        if off:  # another layout adds in another order
+            check(t(), formulas(d, "tanh", 0.7)[k], k)
+        else:
+            assert torch.equal(t(), want[k]), k
+    # without a gradient of h: the next weight's gradient is left as it was
+    before = dv_t()
+    rc = lib.gmm_sm100_post_norm_backward(ptr(c["y"]), ptr(c["x"]), ptr(c["w"]), ptr(c["g"]), ptr(c["v"]), ry, rx,
+                                          ptr(c["dx"]), None, *head, 0.0, dy, dx, dw, dg, None, ws, size, None)
+    assert rc == 0, lib.gmm_sm100_last_error()
+    out.check()
+    assert torch.equal(dx_t(), c["dx"]) and torch.equal(dv_t(), before)
+    check(dy_t(), formulas(d, "tanh", 0.7, use_dh=False)["dy"], "dy")

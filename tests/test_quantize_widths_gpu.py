@@ -1,7 +1,9 @@
-"""Row quantiser at the widths where its shared memory is fullest."""
+"""Row quantiser at the widths where its shared memory is fullest, and at the ends of its buffers."""
 
 import pytest
 import torch
+
+from test_norms_edges_gpu import Guarded, code
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +44,28 @@ def test_expert_weights_of_a_wide_contraction():
     q, s = quantize_experts(w.cuda())
     codes, scale = exact(w.transpose(1, 2).reshape(16, 12640))
     assert torch.equal(s.cpu().flatten(), scale) and torch.equal(q.cpu().view(16, -1), codes)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,dim", [(1, 1), (700, 17), (301, 250), (5, 4096), (3, 16381), (2, 20000)])
+def test_nothing_is_written_outside(T, dim, dtype):
+    from gmm_b200 import capi
+    lib = capi.load()
+    x = torch.randn(T, dim, generator=torch.Generator().manual_seed(2)).to(dtype)
+    c = x.cuda()
+    k = 2
+    place = torch.randperm(T * k, generator=torch.Generator().manual_seed(3)).view(T, k).int()
+    out = Guarded()
+    q, q_t = out.empty((T * k, (dim + 15) // 16 * 16), torch.int8)
+    s, s_t = out.empty((T * k,), torch.float32)
+    dst = place.cuda()
+    rc = lib.gmm_sm100_quantize_rows(c.data_ptr(), code(dtype), T, dim, dst.data_ptr(), k, T * k, q, s, None)
+    assert rc == 0, lib.gmm_sm100_last_error()
+    out.check()
+    codes, scale = exact(x)
+    want = torch.zeros(T * k, (dim + 15) // 16 * 16, dtype=torch.int8)
+    want_s = torch.empty(T * k)
+    for j in range(k):
+        want[place[:, j].long(), :dim] = codes
+        want_s[place[:, j].long()] = scale
+    assert torch.equal(q_t().cpu(), want) and torch.equal(s_t().cpu(), want_s)
