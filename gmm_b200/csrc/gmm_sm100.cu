@@ -943,6 +943,34 @@ __global__ void __launch_bounds__(32) ep_barrier_kernel(const __grid_constant__ 
   }
 }
 
+// Device batch sizes with an empty contraction: the used rows of D become 0, and
+// sizes that cannot be are recorded as the product's kernels record them.
+__global__ void __launch_bounds__(kThreads) zero_rows_kernel(uint4* d, long long row_words, const int32_t* sizes,
+                                                             int experts, long long rows_cap) {
+  __shared__ long long warp_rows[kThreads / 32];
+  long long rows = 0;
+  bool bad = false;
+  for (int e = threadIdx.x; e < experts; e += kThreads) {
+    const int m = sizes[e];
+    bad |= m < 0;
+    rows += max(m, 0);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) rows += __shfl_xor_sync(0xffffffffu, rows, o);
+  if ((threadIdx.x & 31) == 0) warp_rows[threadIdx.x >> 5] = rows;
+  const int bad_any = __syncthreads_or(bad);
+  rows = 0;
+  for (int w = 0; w < kThreads / 32; ++w) rows += warp_rows[w];
+  if (bad_any || rows > rows_cap) {
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+      atomicCAS(&g_device_error, 0, bad_any ? GMM_ERR_INVALID_ARGUMENT : GMM_ERR_BATCH_SUM);
+    return;
+  }
+  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < rows * row_words;
+       i += static_cast<long long>(gridDim.x) * kThreads)
+    d[i] = make_uint4(0, 0, 0, 0);
+}
+
 #include "gmm_pair_kernel.cuh"
 #include "gmm_vark_kernel.cuh"
 #include "gmm_swap_kernel.cuh"
@@ -1642,8 +1670,12 @@ int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_de
   int rc = device_info(dev, &di);
   if (rc != GMM_OK) return rc;
   if (K == 0) {
-    ce = cudaMemsetAsync(D, 0, static_cast<size_t>(T) * N_out * es, stream);
-    return ce == cudaSuccess ? GMM_OK : cuda_fail(ce, "cudaMemsetAsync");
+    const int64_t row_words = N_out * es / 16;
+    const int64_t blocks = std::min<int64_t>((T * row_words + kThreads - 1) / kThreads, 8 * di->sm_count);
+    zero_rows_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(static_cast<uint4*>(D), row_words,
+                                                                            batch_sizes_dev, static_cast<int>(E), T);
+    ce = cudaGetLastError();
+    return ce == cudaSuccess ? GMM_OK : cuda_fail(ce, "empty contraction launch");
   }
   if (!A || !B || !aligned16(A) || !aligned16(B))
     return fail(GMM_ERR_ALIGNMENT, "A and B must be non-null and 16-byte aligned");
