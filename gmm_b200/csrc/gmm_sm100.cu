@@ -1280,7 +1280,7 @@ int launch_stream(const GmmParams& prm, const void* A, const void* B, int64_t K,
 // back to 128 for the SwiGLU and expert-parallel epilogues, which it does not
 // have).
 // 8-bit operands: CTA pairs and 128-row tiles by the same rule, and the
-// streaming kernel when no expert has more than 16 rows and the weights are
+// streaming kernel when no expert has more than 16 rows and the bytes are
 // few (stream_pays), or when "swap" is forced.
 enum TileKind { kTile128 = 0, kTilePair = 1, kTileSwap = 2, kTileStream = 3 };
 
@@ -1303,20 +1303,40 @@ int tile_force() {
 // Whether the streaming kernel can count the tasks of `blocks` row blocks and N columns of B.
 bool stream_fits(int64_t blocks, int64_t N) { return blocks <= INT32_MAX / (N / kStreamCols + 1); }
 
-// Whether few-row experts with `live` weight matrices of N x K bytes go to the
-// streaming kernel: it starts sooner and spreads small problems over every SM,
-// the 128-row tiles keep more of a long stream in flight.  One B200, bf16 out,
-// us, 8 rows an expert, streaming against 128-row tiles:
-//    2 x 768 x 2048 (3 MB)       5.9   9.4     64 x 768 x 2048 (101 MB)  24.7  25.9
-//    8 x 2048 x 1536 (25 MB)    10.5  17.4     96 x 768 x 2048 (151 MB)  33.8  34.6
-//    4 x 7168 x 4096 (117 MB)   27.6  33.5      5 x 7168 x 4096 (147 MB) 41.8  35.7
-//   32 x 768 x 2048 (50 MB)     14.8  17.0    128 x 768 x 2048 (201 MB)  42.2  40.2
-//   40 x 2048 x 1536 (126 MB)   29.4  32.8     64 x 2048 x 1536 (201 MB) 44.4  42.5
-// With 16 rows an expert the token rows cost as much as the weights:
-//   64 x 768 x 2048             29.2  26.8     40 x 2048 x 1536          30.2  32.9
-constexpr double kStreamBytes = 1.3e8;
-bool stream_pays(int64_t live, int64_t K, int64_t N) {
-  return static_cast<double>(live) * static_cast<double>(K) * static_cast<double>(N) <= kStreamBytes;
+// Whether few-row experts with `live` weight matrices of N x K bytes, `rows`
+// token rows in all, go to the streaming kernel: it starts sooner and spreads
+// small problems over every SM, the 128-row tiles keep more of a long stream in
+// flight.  A second block of 8 token rows makes the streaming kernel read as
+// many bytes of tokens as of weights (half with SwiGLU, whose gate and up
+// columns share them): then it keeps only small problems and those whose tiles
+// leave half of the SMs idle.  One B200, bf16 out, us, streaming / 128-row tiles:
+//                                       8 rows an expert      16 rows
+//    2 x 768 x 2048 (3 MB)                  6.1 /  9.4       6.3 /  9.5
+//   16 x 768 x 2048 (25 MB)                 9.9 / 12.1      11.1 / 12.1
+//   32 x 768 x 2048 (50 MB)                15.5 / 17.2      17.4 / 17.6
+//   20 x 2816 x 1024 (58 MB)               19.8 / 19.6      22.9 / 19.8
+//    1 x 4096 x 16384 (67 MB, 64 tiles)    18.3 / 23.6      19.3 / 23.6
+//   32 x 1024 x 2816 (92 MB)               22.7 / 24.2      26.3 / 25.1
+//   64 x 768 x 2048 (101 MB)               24.9 / 26.3      29.2 / 27.0
+//    6 x 4096 x 4096 (101 MB)              25.9 / 26.1      30.0 / 26.1
+//   12 x 2048 x 4096 (101 MB)              25.3 / 27.5      26.3 / 27.8
+//   10 x 5120 x 2048 (105 MB)              30.9 / 27.5      36.4 / 27.8
+//    4 x 7168 x 4096 (117 MB, 64 tiles)    27.5 / 33.5      30.0 / 33.6
+//   16 x 7168 x 1024 (117 MB, 64 tiles)    27.5 / 32.9      30.2 / 33.3
+//   40 x 2048 x 1536 SwiGLU (126 MB)       29.4 / 32.4      30.4 / 32.4
+//    5 x 7168 x 4096 (147 MB)              41.8 / 35.7
+//   96 x 768 x 2048 (151 MB)               33.8 / 34.6
+//   64 x 2048 x 1536 SwiGLU (201 MB)       44.4 / 42.5
+//  128 x 768 x 2048 (201 MB)               42.2 / 40.2
+// (10 x 5120 x 2048 with 8 rows is the streaming kernel's bad case: 1280 tasks
+// for 2368 warps, too many to share in pairs.)
+constexpr double kStreamBytes = 1.3e8, kStreamBytesTwoBlocks = 5e7;
+constexpr int64_t kFewTiles = 74;  // half of the SMs
+bool stream_pays(int64_t live, int64_t rows, int64_t K, int64_t N, bool act) {
+  const double bytes = static_cast<double>(live) * static_cast<double>(K) * static_cast<double>(N);
+  const bool two = !act && rows > 8 * live;
+  if (two && bytes > kStreamBytesTwoBlocks && live > kFewTiles / ((N + 255) / 256)) return false;
+  return bytes <= kStreamBytes;
 }
 
 TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t K, int64_t N, int dtype, int act, bool remote, bool i8) {
@@ -1333,7 +1353,7 @@ TileKind choose_tile_kind(const int64_t* bs, int64_t E, int64_t T, int64_t K, in
     max_m = std::max(max_m, bs[e]);
   }
   if (groups > 0 && T >= 384 * groups) return kTilePair;
-  if (i8 && max_m <= kStreamRows && stream_pays(groups, K, N) && stream_fits(groups, N)) return kTileStream;
+  if (i8 && max_m <= kStreamRows && stream_pays(groups, T, K, N, act) && stream_fits(groups, N)) return kTileStream;
   return (swap_ok && max_m <= 64) ? kTileSwap : kTile128;
 }
 
@@ -1691,7 +1711,7 @@ int forward_dev_impl(const void* A, const void* B, const int32_t* batch_sizes_de
     if (force == GMM_TILE_PAIR) tile_rows = 256;
     else if (force == GMM_TILE_AUTO) {
       if (T >= 384 * E) tile_rows = 256;
-      else few = T <= 16 * E && (!i8 || stream_pays(std::min(E, T), K, N));
+      else few = T <= 16 * E && (!i8 || stream_pays(std::min(E, T), T, K, N, swiglu != 0));
     }
     if (few && i8) tile_rows = stream_fits(E + T / kStreamRows, N) ? kStreamRows : 128;
     else if (few) swap = !swiglu;
