@@ -447,9 +447,10 @@ __device__ __forceinline__ void drain_rows(OutT* const (&rp)[8], int n0, int dim
 
 // The scales one epilogue warp needs for a tile, fetched before it waits for
 // the accumulator: cold reads chunk by chunk during the drain cost more than
-// the rest of it.  One B200, both ways: decode (128 experts, 1..16 rows,
-// 768 x 2048) 61.5 -> 41.1 us; 16384 x 4096 x 14336 on 8 experts 736 -> 633
-// us (3.04 POPS); 4099 rows on 64 experts of 7168 x 4096 331 -> 295 us.
+// the rest of it.  One B200, both ways, a few passes in a graph: decode (128
+// experts, 1..16 rows, 768 x 2048) 61.5 -> 41.1 us; 16384 x 4096 x 14336 on 8
+// experts 736 -> 633 us (calls held at the power cap take 718); 4099 rows on
+// 64 experts of 7168 x 4096 331 -> 295 us.
 struct TileScales {
   float4 c[2];  // accumulator columns 4 * lane .. +3 and 128 + 4 * lane .. +3
   float row;    // lane's row
@@ -498,10 +499,11 @@ __device__ __forceinline__ void drain_slab(const GmmParamsBase& p, const TableVi
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
-// The same with a fast reciprocal (2 * 2^-24 instead of a correctly rounded
-// quotient, far below the 16-bit output's step), for the 8-bit kinds: their
-// mainloop is half as long, and the division kept their epilogue from hiding
-// behind it.
+// The same with a fast reciprocal, for the 8-bit kinds: their mainloop is half
+// as long, and the division kept their epilogue from hiding behind it.  It is
+// within 2 ulp (4 * 2^-24 of the value) instead of half an ulp, and 0 past
+// 2^126 (gates below -87), beside the exponential's 2 + 1.173 |g| ulp: far
+// below the 16-bit output's step.
 __device__ __forceinline__ float silu_mul_fast(float g, float u) { return g * __fdividef(1.0f, 1.0f + __expf(-g)) * u; }
 
 // SwiGLU variant of drain_slab: TMEM columns [0, 128) hold the tile's gate

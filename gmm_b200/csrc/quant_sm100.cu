@@ -16,7 +16,6 @@
 // shared-memory ring and leave as one bulk store a place.
 
 #include <algorithm>
-#include <cstdio>
 
 #include "gmm_sm100.h"
 #include "row_ring.cuh"

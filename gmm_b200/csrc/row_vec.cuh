@@ -119,19 +119,4 @@ __device__ __forceinline__ Raw8<T> load8(const T* row, int col, int dim) {
   }
 }
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void store8(T* row, int col, int dim, const float (&f)[8]) {
-  if constexpr (kVec) {
-    if (col >= dim) return;
-    const Raw8<T> r = pack<T>(f);
-    uint4* p = reinterpret_cast<uint4*>(row + col);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) p[i] = r.q[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < dim) row[col + i] = from_float<T>(f[i]);
-  }
-}
-
 }  // namespace gmm_sm100
