@@ -288,7 +288,7 @@ NormArgs check_norm(const OptTensor& y, const at::Tensor& x, const OptTensor& we
     token.back() = 1;
     if (gate->sizes() == x.sizes() && x.dim() > 1) n.gate_mode = GMM_GATE_MODE_FULL;
     else if (gate->dim() == 1 && gate->size(0) == n.dim) n.gate_mode = GMM_GATE_MODE_CHANNEL;
-    else if (x.dim() > 1 && gate->sizes() == c10::IntArrayRef(token)) n.gate_mode = GMM_GATE_MODE_TOKEN;
+    else if (gate->sizes() == c10::IntArrayRef(token)) n.gate_mode = GMM_GATE_MODE_TOKEN;
     else TORCH_CHECK(false, "gate must have shape [dim], [..., 1] or [..., dim], got ", gate->sizes());
   }
   TORCH_CHECK(gmm_sm100_check_device(x.get_device()) == GMM_OK, "post_norm: ", gmm_sm100_last_error());

@@ -143,6 +143,22 @@ def test_no_slope_at_infinite_gates(gate, kind):
     assert (dg[at] == 0).all() and not dg.isnan().any()
 
 
+@pytest.mark.parametrize("D", [1, 24])
+def test_a_token_gate_of_one_row_without_batch_dimensions(D):
+    """[..., 1] with no leading dimension is [1]."""
+    from gmm_b200.norms import post_norm
+    d = inputs(1, D, torch.float32, gate="token", following=False, seed=33)
+    want = formulas(d, "sigmoid", 0.6)
+    c = cuda(d)
+    leaves = {k: (c[k][0] if k != "w" else c[k]).detach().clone().requires_grad_() for k in ("y", "x", "w", "g")}
+    new = post_norm(leaves["y"], leaves["x"], leaves["w"], gate=leaves["g"], gate_act="sigmoid", residual_scale=0.6)
+    grads = torch.autograd.grad(new, list(leaves.values()), c["dx"][0])
+    check(new, (want["new"][0][0], want["new"][1][0]), "new")
+    for k, gr in zip(leaves, grads):
+        value, bound = want["d" + k]
+        check(gr, (value.reshape(gr.shape), bound.reshape(gr.shape)), k)
+
+
 # ------------------------------------------------------------------ the ends of the buffers
 GUARD = 512
 FILL = 0xA5
