@@ -65,7 +65,8 @@ def quantize_experts(w: torch.Tensor, trans_b: bool = False) -> Tuple[torch.Tens
         raise RuntimeError("w must be 3D [num_experts, dim, dim_out] (or [num_experts, dim_out, dim])")
     rows = w if trans_b else w.transpose(1, 2)
     E, n, dim = rows.shape
-    q, scale = quantize_rows(rows.reshape(E * n, dim))
+    with torch.no_grad():  # of parameters too: the scales are data, not a function of them
+        q, scale = quantize_rows(rows.reshape(E * n, dim))
     return q.view(E, n, q.shape[1]), scale.view(E, n)
 
 

@@ -98,3 +98,12 @@ def test_a_block_refuses_forward_gradients(which):
         t[which] = fwAD.make_dual(t[which], torch.empty_like(t[which]))
         with pytest.raises(RuntimeError, match="no backward pass"):
             block(t)
+
+
+def test_quantised_parameters_carry_no_graph():
+    """The codes and scales of parameters go into a block like any others."""
+    from gmm_b200.int8 import quantize_experts
+    with FakeTensorMode():
+        w = torch.empty(4, 48, 64, device="cuda", requires_grad=True)
+        for t in quantize_experts(w) + quantize_experts(w, trans_b=True):
+            assert not t.requires_grad and t.grad_fn is None
