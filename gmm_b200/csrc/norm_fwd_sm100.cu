@@ -15,7 +15,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
   RowRing<3, kLayout == kWhole> ring;
   ring.input(0, p.x, sizeof(T), D, D);
   ring.input(1, p.y, sizeof(T), kMode == kPreNorm ? 0 : D, D);
-  ring.input(2, p.gate, sizeof(G), is_full(kMode) ? D : 0, D);
+  // The element size from the call: as a constant it lets the compiler merge the
+  // inputs' addressing, at the price of spills (8192 x 6144 bf16, 89 -> 104 us).
+  ring.input(2, p.gate, p.gate_f32 ? 4 : sizeof(T), is_full(kMode) ? D : 0, D);
   ring.start(smem, slots, p.rows, gate_pad(kLayout, kMode));
   if (threadIdx.x < 32)
 #pragma unroll
@@ -74,9 +76,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) norm_fwd_ring_kernel(const 
           for (int j = 0; j < V; ++j) g[j] = 0.f;
           if (c < units) read_param<G, V>(gs, c, g);
           if (kLayout == kShifted) span.mask(c, g);
-          act_of<sizeof(G) == 2, false, V>(g, p.act);
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[i * V + j] *= g[j];
+          for (int j = 0; j < V; ++j) {
+            act_of<sizeof(G) == 2, false, 1>(g + j, p.act);
+            y[i * V + j] *= g[j];
+          }
         }
       }
       const float ry = rsqrtf(block_sum(sq[0] + sq[1], scratch[0][odd]) * inv_d + p.eps);

@@ -82,7 +82,7 @@ struct NormParams {
 
 // g[j] = act(g[j]) and, with kSlope, slope[j] = act'(g[j]); one branch for all
 // N, so that their exponentials overlap.  With e = exp(-|g|), r = 1 / (1 + e):
-//   sigmoid  r or e r by the sign of g, slope e r^2  (without kSlope from exp(-g) alone)
+//   sigmoid  r or e r by the sign of g, slope e r^2  (kFast without kSlope: from exp(-g) alone)
 //   tanh     slope 4 e r^2 with e = exp(-2 |g|)
 // Slopes from a (1 - a) or 1 - a^2 would lose a saturated gate's to the
 // rounding of a.
@@ -92,14 +92,18 @@ struct NormParams {
 // 2^-23 of a value): the sigmoid (10 + 2.35 |g|) * 2^-24 and the slopes, twice
 // the reciprocal and twice the argument for tanh, below (20 + 4.7 |g|) * 2^-24,
 // less than a half step of 16 bits (results below 2^-126 may be 0).  expf
-// and a correctly rounded reciprocal made such a gate cost more than its rows'
-// bytes (8191 x 6144 fp16 forward: 111 us against 70); fp32 rows have twice the
+// and a division made such a gate cost more than its rows' bytes (8191 x 6144
+// fp16 forward: 111 us against 70); fp32 rows have twice the
 // bytes to hide them, and gates shared by rows or elements are few.
 template <bool kFast, bool kSlope, int N>
 __device__ __forceinline__ void act_of(float* g, int act, float* slope = nullptr) {
+  // e = exp(x) and 1 / (1 + e); kFast for any x, else for x <= 0: 1 + e is in
+  // [1, 2] then, and one step of Newton and Raphson on the fast reciprocal leaves
+  // its last rounding, without the division's path for numbers out of range.
   auto ratio = [](float x, float& e) {
     e = kFast ? __expf(x) : expf(x);
-    return kFast ? __fdividef(1.f, 1.f + e) : __frcp_rn(1.f + e);
+    const float d = 1.f + e, r = __fdividef(1.f, d);
+    return kFast ? r : fmaf(r, fmaf(-d, r, 1.f), r);
   };
   if (act == GMM_GATE_TANH) {
 #pragma unroll
@@ -115,12 +119,12 @@ __device__ __forceinline__ void act_of(float* g, int act, float* slope = nullptr
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       float e;
-      if constexpr (kSlope) {
-        const float r = ratio(-fabsf(g[j]), e), er = e * r;
-        slope[j] = er * r;
-        g[j] = g[j] >= 0.f ? r : er;
-      } else {
+      if constexpr (kFast && !kSlope) {
         g[j] = ratio(-g[j], e);
+      } else {
+        const float r = ratio(-fabsf(g[j]), e), er = e * r;
+        if constexpr (kSlope) slope[j] = er * r;
+        g[j] = g[j] >= 0.f ? r : er;
       }
     }
   } else if constexpr (kSlope) {
@@ -383,15 +387,18 @@ __device__ __forceinline__ void row_params(const NormParams& p, const Span<V, kL
 #pragma unroll
   for (int i = 0; i < kE / V; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
-    if constexpr (kMode == kSharedGate)
-      if (channel) act_of<false, false, V>(g + i * V, p.act);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const bool in = span.has(c, j);
       const int e = i * V + j;
       if (kMode != kPreNorm) {
         pw[e] = in ? (pw[e] + p.offset) * p.scale : 0.f;
-        if (kMode == kSharedGate && channel) pw[e] *= g[e];
+        if constexpr (kMode == kSharedGate) {
+          if (channel) {
+            act_of<false, false, 1>(g + e, p.act);
+            pw[e] *= g[e];
+          }
+        }
       }
       vo[e] = in && with_v ? vo[e] + p.offset : 0.f;
     }
