@@ -16,6 +16,7 @@ int current_sm_count(int* sms) { *sms = 148; return 0; }
 """
 
 GATE = r"""
+#include <cstdio>
 #include "norm_sm100.cuh"
 using namespace gmm_sm100;
 // The words an fp32 gate's row is read in beside 16-bit rows that start `shift` elements into their first unit of
@@ -41,6 +42,7 @@ int main() {
 """
 
 QUANT = r"""
+#include <cstdio>
 #include "quant_sm100.cu"
 using namespace gmm_sm100;
 // Every width and type of the quantiser's ring asks for no more than a block may have, and its blocks for no more than
@@ -59,6 +61,7 @@ int main() {
 """
 
 NORM = r"""
+#include <cstdio>
 #include "norm_sm100.cuh"
 using namespace gmm_sm100;
 // The same of the norms: rows of one to five inputs, the last an fp32 gate's where there is one.
